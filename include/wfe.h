@@ -222,6 +222,76 @@ int wfe_augment_waveform(wfe_handle h, const float* wav, const int64_t* offsets,
 int wfe_power_spectrum(wfe_handle h, const float* wav, const int64_t* offsets, const int32_t* lengths,
                        int64_t row_stride, int32_t batch, int32_t n_samples, float* out, void* stream);
 
+/* ---- the decoder's vocabulary matrix ----------------------------------------- */
+/* The two operators at the ends of the decoder, where the collator's labels meet the vocabulary matrix W
+ * (vocab, dim): the loss of WhisperForConditionalGeneration (proj_out and the cross entropy, as the Trainer of
+ * finetune.py:143 / finetune_all.py calls it) and the embedding of its input tokens.
+ * They take no handle: every call names its device and gets its workspace from the caller, so that calls on
+ * different streams, from different threads or in different captured graphs share nothing.  Errors: a negative
+ * wfe_status, its text in wfe_last_error(NULL) of the same thread.  Nothing is allocated, nothing synchronises,
+ * results are the same bits from run to run. */
+typedef enum { WFE_F32 = 0, WFE_F16 = 1, WFE_BF16 = 2 } wfe_dtype;
+typedef enum { WFE_REDUCE_NONE = 0, WFE_REDUCE_SUM = 1, WFE_REDUCE_MEAN = 2 } wfe_reduction;
+#define WFE_GRAD_HIDDEN 1
+#define WFE_GRAD_WEIGHT 2
+
+/* Softmax cross entropy of labels under logits = hidden @ W^T, the logits never kept:
+ *   loss_n = log sum_v exp(h_n . W_v) - h_n . W_{y_n}     (0 where y_n == ignore_index, whatever h_n holds)
+ * computed with float32 logits and sums.  A label outside 0..vocab-1 that is not ignore_index makes the loss NaN.
+ * Hidden row n lies at hidden + (n / inner) * outer_stride + (n % inner) * inner_stride (elements), so that a
+ * (batch, length, dim) view is taken as it is; rows of W at weight + v * weight_stride.  dim is contiguous. */
+typedef struct {
+  int32_t device;
+  int32_t dtype;            /* wfe_dtype of hidden and weight */
+  int64_t rows;             /* tokens, 0..2^24 */
+  int64_t inner;            /* rows per outer step; `rows` when there is one stride only */
+  int64_t outer_stride, inner_stride, weight_stride;
+  int32_t dim;              /* 1..16384 */
+  int32_t vocab;            /* 1..2^24 */
+  int32_t label_bits;       /* 32 or 64 */
+  int32_t reduction;        /* wfe_reduction: loss has `rows` entries, or one */
+  int64_t ignore_index;
+  int32_t grad_hidden_dtype, grad_weight_dtype;   /* WFE_F32 or `dtype` */
+} wfe_linear_ce;
+
+/* Bytes of the state that the forward pass leaves for the backward pass, and of the workspace of either pass (grads:
+ * WFE_GRAD_ bits of the backward pass; weight: the address the pass will get, read by nobody -- rows of W that are
+ * no whole multiples of 128 bytes, or not 16-byte aligned, are copied into the workspace).  Both start on 16 bytes.
+ * Negative: a bad description. */
+int64_t wfe_linear_ce_state_bytes(const wfe_linear_ce* d);
+int64_t wfe_linear_ce_workspace_bytes(const wfe_linear_ce* d, const void* weight, int32_t backward, int32_t grads);
+/* loss: float32, `rows` entries (WFE_REDUCE_NONE) or one.  With no kept row the mean is NaN and the sum 0. */
+int wfe_linear_ce_forward(const wfe_linear_ce* d, const void* hidden, const void* weight, const void* labels,
+                          float* loss, void* state, void* workspace, int64_t workspace_bytes, void* stream);
+/* upstream: float32 gradient of `loss` (as many entries as it).  grad_hidden (rows, dim) and grad_weight
+ * (vocab, dim), contiguous, fully overwritten; either may be NULL.  hidden, weight and state as in the forward pass. */
+int wfe_linear_ce_backward(const wfe_linear_ce* d, const void* hidden, const void* weight, const void* state,
+                           const float* upstream, void* grad_hidden, void* grad_weight, void* workspace,
+                           int64_t workspace_bytes, void* stream);
+
+/* out_n = scale * W_{ids_n}, rounded once; a row of NaN for an id outside 0..vocab-1.  The gradient of W is
+ * scale * (sum of grad_out_n over the n with ids_n = v, in float32 and in the order of n), zero for padding_idx and for
+ * tokens that do not occur; ids outside the range give nothing. */
+typedef struct {
+  int32_t device;
+  int32_t dtype;            /* wfe_dtype of weight, out and grad_out */
+  int64_t rows;             /* tokens, 0..2^24 */
+  int64_t weight_stride;    /* elements */
+  int64_t grad_stride;      /* row stride of grad_out, elements; 0: every row is the same */
+  int32_t dim;              /* 1..16384 */
+  int32_t vocab;            /* 1..2^24 */
+  int32_t id_bits;          /* 32 or 64 */
+  int32_t grad_weight_dtype;   /* WFE_F32 or `dtype` */
+  int64_t padding_idx;      /* negative: none */
+  float scale;
+} wfe_embedding_desc;
+
+int wfe_embedding(const wfe_embedding_desc* d, const void* ids, const void* weight, void* out, void* stream);
+int64_t wfe_embedding_workspace_bytes(const wfe_embedding_desc* d);
+/* grad_weight (vocab, dim) contiguous, fully overwritten. */
+int wfe_embedding_backward(const wfe_embedding_desc* d, const void* ids, const void* grad_out, void* grad_weight,
+                           void* workspace, int64_t workspace_bytes, void* stream);
+
 /* ---- output element type ---------------------------------------------------- */
 /* No reference counterpart: the reference's extractor returns float32 and the
  * Trainer casts input_features to the training dtype on the device (fp16=True,

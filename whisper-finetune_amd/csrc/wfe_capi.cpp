@@ -15,6 +15,7 @@
 #include <vector>
 
 #include "../../include/wfe.h"
+#include "wfe_capi_util.h"
 #include "wfe_kernels.h"
 #include "wfe_layout.h"
 
@@ -95,15 +96,7 @@ constexpr size_t kInitOps = (size_t)kMaxBatchPerLaunch * 4;
 constexpr size_t kInitNoise = 1024;
 constexpr size_t kMaxTimedLaunches = 1 << 16;    // event triples kept while wfe_kernel_timing is on
 
-int fail(wfe_context* h, int code, const char* fmt, ...) {
-  char buf[512];
-  va_list ap;
-  va_start(ap, fmt);
-  vsnprintf(buf, sizeof buf, fmt, ap);
-  va_end(ap);
-  if (h) h->err = buf; else g_create_err = buf;
-  return code;
-}
+using wfe::fail;
 
 #define HIP_TRY(h, expr)                                                                 \
   do {                                                                                   \
@@ -111,18 +104,7 @@ int fail(wfe_context* h, int code, const char* fmt, ...) {
     if (e_ != hipSuccess) return fail(h, WFE_ERR_HIP, "%s: %s", #expr, hipGetErrorString(e_)); \
   } while (0)
 
-struct DeviceGuard {
-  int prev = -1;
-  bool ok = true;
-  explicit DeviceGuard(int dev) {
-    if (hipGetDevice(&prev) != hipSuccess) prev = -1;
-    if (prev != dev) ok = hipSetDevice(dev) == hipSuccess;
-  }
-  ~DeviceGuard() {
-    int cur = -1;
-    if (prev >= 0 && hipGetDevice(&cur) == hipSuccess && cur != prev) (void)hipSetDevice(prev);
-  }
-};
+using wfe::DeviceGuard;
 
 int check_common(wfe_context* h, const void* wav, const int32_t* lengths, int32_t batch, int32_t n_samples,
                  const void* out) {
@@ -334,6 +316,16 @@ int run_frontend(wfe_context* h, const void* wav, int channels, const int64_t* o
 }
 
 }  // namespace
+
+int wfe::fail(wfe_context* h, int code, const char* fmt, ...) {
+  char buf[512];
+  va_list ap;
+  va_start(ap, fmt);
+  vsnprintf(buf, sizeof buf, fmt, ap);
+  va_end(ap);
+  if (h) h->err = buf; else g_create_err = buf;
+  return code;
+}
 
 extern "C" {
 

@@ -28,6 +28,19 @@ class WfeAugOp(C.Structure):
                 ("f0", C.c_float), ("f1", C.c_float), ("d0", C.c_double)]
 
 
+class WfeLinearCe(C.Structure):
+    _fields_ = [("device", C.c_int32), ("dtype", C.c_int32), ("rows", C.c_int64), ("inner", C.c_int64),
+                ("outer_stride", C.c_int64), ("inner_stride", C.c_int64), ("weight_stride", C.c_int64),
+                ("dim", C.c_int32), ("vocab", C.c_int32), ("label_bits", C.c_int32), ("reduction", C.c_int32),
+                ("ignore_index", C.c_int64), ("grad_hidden_dtype", C.c_int32), ("grad_weight_dtype", C.c_int32)]
+
+
+class WfeEmbedding(C.Structure):
+    _fields_ = [("device", C.c_int32), ("dtype", C.c_int32), ("rows", C.c_int64), ("weight_stride", C.c_int64),
+                ("grad_stride", C.c_int64), ("dim", C.c_int32), ("vocab", C.c_int32), ("id_bits", C.c_int32),
+                ("grad_weight_dtype", C.c_int32), ("padding_idx", C.c_int64), ("scale", C.c_float)]
+
+
 AUG_SPEED, AUG_SHIFT, AUG_VOLUME, AUG_NOISE, AUG_AFFINE = 1, 2, 3, 4, 5
 ERR_ARG, ERR_HIP, ERR_ALLOC, ERR_SAMPLING = -1, -2, -3, -4
 
@@ -54,6 +67,13 @@ SYMBOLS = {
                                        _P, _P, C.c_int32, _P, _P, _P]),
     "wfe_noise_bank_changed": (C.c_int, [_P]),
     "wfe_set_output_format": (C.c_int, [_P, C.c_int32]),
+    "wfe_linear_ce_state_bytes": (C.c_int64, [_P]),
+    "wfe_linear_ce_workspace_bytes": (C.c_int64, [_P, _P, C.c_int32, C.c_int32]),
+    "wfe_linear_ce_forward": (C.c_int, [_P, _P, _P, _P, _P, _P, _P, C.c_int64, _P]),
+    "wfe_linear_ce_backward": (C.c_int, [_P, _P, _P, _P, _P, _P, _P, _P, C.c_int64, _P]),
+    "wfe_embedding": (C.c_int, [_P, _P, _P, _P, _P]),
+    "wfe_embedding_workspace_bytes": (C.c_int64, [_P]),
+    "wfe_embedding_backward": (C.c_int, [_P, _P, _P, _P, _P, C.c_int64, _P]),
     "wfe_kernel_timing": (C.c_int, [_P, C.c_int32]),
     "wfe_kernel_times": (C.c_int, [_P, C.POINTER(C.c_double), C.POINTER(C.c_double), C.POINTER(C.c_int64)]),
     "wfe_dft_table_floats": (C.c_int64, []),

@@ -19,6 +19,10 @@ What it does, in this process and before anything touches a GPU:
   * with ``WFE_INSTALL_EXTRACTOR=1``, ``WhisperProcessor.from_pretrained`` returns a
     processor whose feature extractor is the MI355X one (infer_tfs.py:27-37, evaluation.py:41-46).
 
+  * with ``WFE_INSTALL_DECODER=1``, ``WhisperForConditionalGeneration.from_pretrained`` returns a model whose token
+    embedding and training loss are the HIP operators of ``wfe_amd.decoder`` (finetune.py:57-62, finetune_all.py:57-62):
+    the logits of a training step are never kept.
+
   * for scripts that use the front end: ``WFE_DEVICE_OUTPUT`` defaults to 1 and
     ``Seq2SeqTrainingArguments`` / ``TrainingArguments`` default to ``dataloader_pin_memory=False`` (the
     reference never sets it, finetune.py:111-133), so ``input_features`` stay on the GPU instead of going
@@ -123,6 +127,19 @@ def _install_extractor_hook() -> None:
     WhisperProcessor.from_pretrained = classmethod(from_pretrained)
 
 
+def _install_decoder_hook() -> None:
+    from transformers import WhisperForConditionalGeneration
+    from .decoder import install
+    original = WhisperForConditionalGeneration.from_pretrained.__func__
+
+    def from_pretrained(cls, *args, **kwargs):
+        out = original(cls, *args, **kwargs)
+        if isinstance(out, tuple):              # output_loading_info=True
+            return (install(out[0]), *out[1:])
+        return install(out)
+    WhisperForConditionalGeneration.from_pretrained = classmethod(from_pretrained)
+
+
 def _install_training_defaults(note=sys.stderr) -> None:
     """dataloader_pin_memory=False by default (CUDA tensors cannot be pinned) and the two keyword renames of
     newer transformers releases.  Best effort: without transformers there is nothing to patch."""
@@ -178,6 +195,8 @@ def main(argv=None) -> None:
     install_redirect()
     if os.environ.get("WFE_INSTALL_EXTRACTOR", "0") == "1":
         _install_extractor_hook()
+    if os.environ.get("WFE_INSTALL_DECODER", "0") == "1":
+        _install_decoder_hook()
     # as `python script.py`: the script's directory leads sys.path, argv[0] is the script
     script_dir = os.path.dirname(script)
     sys.path.insert(0, script_dir)               # (-m put the cwd first; the script's directory goes ahead of it)
