@@ -13,7 +13,7 @@ constexpr int kLceRowPad = 256;     // packed hidden rows are padded to this man
 
 // What the forward pass leaves for the backward pass, `rows` entries each; r counts kept rows, n all rows.
 struct LceState {
-  int* head;         // [0] kept rows, [1] ticket of the reduction
+  int* head;         // [0] kept rows
   int* index;        // n of kept row r, ascending
   int* label;        // label of kept row r; -1: outside 0..vocab-1
   float* lse;        // log sum exp of its logits

@@ -34,24 +34,27 @@ struct Vec {
   }
 };
 
-// One wave per token.
+// One wave per token and slab of columns: few tokens still make many waves, and no wave waits for a second load.
 template <typename T>
 __global__ __launch_bounds__(256) void embed_kernel(const void* ids, int id_bits, long long rows, const T* weight,
                                                     long long ld, int dim, int vocab, float scale, T* out) {
-  const long long n = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+  constexpr int kSlab = 64 * Vec<T>::kN;
+  const unsigned slabs = (unsigned)(dim + kSlab - 1) / kSlab;
+  const unsigned long long wave = (unsigned long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const long long n = (long long)(wave / slabs);
   if (n >= rows) return;
   const long long id = id_at(ids, id_bits, n);
   const bool known = id >= 0 && id < vocab;
   const T* in = weight + (known ? id : 0) * ld;
   T* to = out + n * dim;
   const bool wide = ((reinterpret_cast<uintptr_t>(in) | reinterpret_cast<uintptr_t>(to)) & 15) == 0;
-  for (int d = (threadIdx.x & 63) * Vec<T>::kN; d < dim; d += 64 * Vec<T>::kN) {
-    Vec<T> v;
-    v.load(in + d, dim - d, wide);
-    for (int e = 0; e < Vec<T>::kN; ++e)
-      v.x[e] = known ? static_cast<T>(static_cast<float>(v.x[e]) * scale) : static_cast<T>(__builtin_nanf(""));
-    v.store(to + d, dim - d, wide);
-  }
+  const int d = (int)(wave % slabs) * kSlab + (threadIdx.x & 63) * Vec<T>::kN;
+  if (d >= dim) return;
+  Vec<T> v;
+  v.load(in + d, dim - d, wide);
+  for (int e = 0; e < Vec<T>::kN; ++e)
+    v.x[e] = known ? static_cast<T>(static_cast<float>(v.x[e]) * scale) : static_cast<T>(__builtin_nanf(""));
+  v.store(to + d, dim - d, wide);
 }
 
 // ---- the gradient ---------------------------------------------------------------------------------------
@@ -124,40 +127,149 @@ __global__ __launch_bounds__(kSortWaves * 64) void embed_sort_kernel(const void*
   }
 }
 
-// One wave per row of the vocabulary.
+// The sums.  Rows of the vocabulary with at most kPiece tokens ("light") are summed and written by one wave; a
+// common token's list ("heavy") is cut at multiples of kPiece positions of the sorted list, each piece is summed by one wave
+// to float32 partial sums, and embed_join_kernel adds them up in order.  A piece holds parts of at most two heavy rows:
+// slot 0 is the one at its first position, slot 1 one that begins behind it.
+constexpr int kPiece = 64, kRowsPerWave = 8, kJoinWaves = 16;
+
+struct SumArgs {
+  const int* start;
+  const int* order;
+  const void* ids;
+  int id_bits;
+  const void* grad;
+  long long ld;
+  long long rows;
+  int dim, vocab;
+  float scale;
+  void* out;
+  int out_f32;
+  float* partial;         // (pieces, 2, dim)
+};
+
 template <typename T>
-__global__ __launch_bounds__(256) void embed_sum_kernel(const int* start, const int* order, const T* grad,
-                                                        long long ld, int dim, int vocab, float scale, void* out,
-                                                        int out_f32) {
-  const int v = blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (v >= vocab) return;
-  const int first = start[v], last = start[v + 1];
-  constexpr int kN = Vec<T>::kN;
-  const bool wide = (reinterpret_cast<uintptr_t>(grad) & 15) == 0 && (ld * (long long)sizeof(T)) % 16 == 0;
-  for (int d = (threadIdx.x & 63) * kN; d < dim; d += 64 * kN) {
-    float sum[kN];
-    for (int e = 0; e < kN; ++e) sum[e] = 0.f;
-    for (int i = first; i < last; ++i) {
-      Vec<T> x;
-      x.load(grad + (long long)order[i] * ld + d, dim - d, wide);
-      for (int e = 0; e < kN; ++e) sum[e] += static_cast<float>(x.x[e]);
-    }
-    const long long at = (long long)v * dim + d;
-    if (out_f32) {
-      float* to = static_cast<float*>(out) + at;
-      for (int e = 0; e < kN && d + e < dim; ++e) to[e] = sum[e] * scale;
-    } else {
-      Vec<T> x;
-      for (int e = 0; e < kN; ++e) x.x[e] = static_cast<T>(sum[e] * scale);
-      T* to = static_cast<T*>(out) + at;
-      x.store(to, dim - d, (reinterpret_cast<uintptr_t>(to) & 15) == 0);
-    }
+__device__ inline void add_rows(float* sum, const int* order, int first, int last, const T* grad, long long ld, int d,
+                                int left, bool wide) {
+  constexpr int kN = Vec<T>::kN, kDeep = 8;
+  int i = first;
+  for (; i + kDeep <= last; i += kDeep) {       // kDeep rows in flight
+    Vec<T> x[kDeep];
+#pragma unroll
+    for (int k = 0; k < kDeep; ++k) x[k].load(grad + (long long)order[i + k] * ld + d, left, wide);
+#pragma unroll
+    for (int k = 0; k < kDeep; ++k)
+#pragma unroll
+      for (int e = 0; e < kN; ++e) sum[e] += static_cast<float>(x[k].x[e]);
+  }
+  for (; i < last; ++i) {
+    Vec<T> x;
+    x.load(grad + (long long)order[i] * ld + d, left, wide);
+#pragma unroll
+    for (int e = 0; e < kN; ++e) sum[e] += static_cast<float>(x.x[e]);
   }
 }
 
 template <typename T>
+__device__ inline void write_sum(const float* sum, const SumArgs& p, int v, int d) {
+  constexpr int kN = Vec<T>::kN;
+  const long long at = (long long)v * p.dim + d;
+  if (p.out_f32) {
+    float* to = static_cast<float*>(p.out) + at;
+    const bool wide = (reinterpret_cast<uintptr_t>(to) & 15) == 0;
+#pragma unroll
+    for (int h = 0; h < kN; h += 4) {
+      Vec<float> x;
+      for (int e = 0; e < 4; ++e) x.x[e] = sum[h + e] * p.scale;
+      if (d + h < p.dim) x.store(to + h, p.dim - d - h, wide);
+    }
+  } else {
+    Vec<T> x;
+#pragma unroll
+    for (int e = 0; e < kN; ++e) x.x[e] = static_cast<T>(sum[e] * p.scale);
+    T* to = static_cast<T*>(p.out) + at;
+    x.store(to, p.dim - d, (reinterpret_cast<uintptr_t>(to) & 15) == 0);
+  }
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void embed_sum_kernel(const SumArgs p, int piece_blocks) {
+  constexpr int kN = Vec<T>::kN, kSlab = 64 * kN;
+  const int lane = threadIdx.x & 63;
+  const T* grad = static_cast<const T*>(p.grad);
+  const bool wide = (reinterpret_cast<uintptr_t>(grad) & 15) == 0 && (p.ld * (long long)sizeof(T)) % 16 == 0;
+  if ((int)blockIdx.x < piece_blocks) {
+    const int slabs = (p.dim + kSlab - 1) / kSlab;
+    const int wave = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));
+    const int piece = wave / slabs, d = (wave % slabs) * kSlab + lane * kN;
+    const int total = p.start[p.vocab], i0 = piece * kPiece, i1 = min(i0 + kPiece, total);
+    if (i0 >= total || d >= p.dim) return;
+    const int v0 = (int)id_at(p.ids, p.id_bits, p.order[i0]), v1 = (int)id_at(p.ids, p.id_bits, p.order[i1 - 1]);
+    for (int slot = 0; slot < 2; ++slot) {
+      const int v = slot ? v1 : v0;
+      if (slot && v1 == v0) break;
+      const int first = p.start[v], last = p.start[v + 1];
+      if (last - first <= kPiece) continue;
+      float sum[kN];
+      for (int e = 0; e < kN; ++e) sum[e] = 0.f;
+      add_rows<T>(sum, p.order, max(first, i0), min(last, i1), grad, p.ld, d, p.dim - d, wide);
+      float* to = p.partial + ((long long)piece * 2 + slot) * p.dim + d;
+      for (int e = 0; e < kN && d + e < p.dim; ++e) to[e] = sum[e];
+    }
+    return;
+  }
+  const int v0 = __builtin_amdgcn_readfirstlane(((blockIdx.x - piece_blocks) * 4 + (threadIdx.x >> 6)) * kRowsPerWave);
+  if (v0 >= p.vocab) return;
+  const int bounds = lane <= kRowsPerWave ? p.start[min(v0 + lane, p.vocab)] : 0;
+  for (int k = 0; k < kRowsPerWave && v0 + k < p.vocab; ++k) {
+    const int first = __builtin_amdgcn_readlane(bounds, k), last = __builtin_amdgcn_readlane(bounds, k + 1);
+    if (last - first > kPiece) continue;
+    for (int d = lane * kN; d < p.dim; d += kSlab) {
+      float sum[kN];
+      for (int e = 0; e < kN; ++e) sum[e] = 0.f;
+      add_rows<T>(sum, p.order, first, last, grad, p.ld, d, p.dim - d, wide);
+      write_sum<T>(sum, p, v0 + k, d);
+    }
+  }
+}
+
+// One block per piece (in which a heavy row may begin) and slab; the row's partial sums go to the waves in turns of
+// contiguous runs, then the waves' sums are added in order.
+template <typename T>
+__global__ __launch_bounds__(kJoinWaves * 64) void embed_join_kernel(const SumArgs p) {
+  constexpr int kN = Vec<T>::kN, kSlab = 64 * kN;
+  __shared__ float sums[kJoinWaves][kSlab];
+  const int slabs = (p.dim + kSlab - 1) / kSlab;
+  const int piece = blockIdx.x / slabs, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int d = (blockIdx.x % slabs) * kSlab + lane * kN;
+  const int total = p.start[p.vocab], i0 = piece * kPiece, i1 = min(i0 + kPiece, total);
+  if (i0 >= total) return;
+  const int v = (int)id_at(p.ids, p.id_bits, p.order[i1 - 1]);
+  const int first = p.start[v], last = p.start[v + 1];
+  if (last - first <= kPiece || first < i0) return;
+  const int pieces = (last - 1) / kPiece - piece + 1;
+  const int each = (pieces + kJoinWaves - 1) / kJoinWaves;
+  float sum[kN];
+  for (int e = 0; e < kN; ++e) sum[e] = 0.f;
+  if (d < p.dim)
+    for (int i = wave * each; i < min((wave + 1) * each, pieces); ++i) {
+      const float* from = p.partial + ((long long)(piece + i) * 2 + (i == 0 && first > i0)) * p.dim + d;
+      for (int e = 0; e < kN; ++e) sum[e] += d + e < p.dim ? from[e] : 0.f;
+    }
+  for (int e = 0; e < kN; ++e) sums[wave][lane * kN + e] = sum[e];
+  __syncthreads();
+  if (wave > 0 || d >= p.dim) return;
+  for (int w = 1; w < kJoinWaves; ++w)
+    for (int e = 0; e < kN; ++e) sum[e] += sums[w][lane * kN + e];
+  write_sum<T>(sum, p, v, d);
+}
+
+int64_t index_bytes(const wfe_embedding_desc& d) { return 4 * ((int64_t)d.vocab + 1 + d.rows + 15) / 64 * 64 + 64; }
+
+template <typename T>
 hipError_t embed(const wfe_embedding_desc& d, const void* ids, const void* weight, void* out, hipStream_t stream) {
-  embed_kernel<T><<<dim3((unsigned)((d.rows + 3) / 4)), dim3(256), 0, stream>>>(
+  const int64_t slabs = (d.dim + 64 * Vec<T>::kN - 1) / (64 * Vec<T>::kN);
+  embed_kernel<T><<<dim3((unsigned)((d.rows * slabs + 3) / 4)), dim3(256), 0, stream>>>(
       ids, d.id_bits, d.rows, static_cast<const T*>(weight), d.weight_stride, d.dim, d.vocab, d.scale,
       static_cast<T*>(out));
   return hipGetLastError();
@@ -170,17 +282,39 @@ hipError_t embed_backward(const wfe_embedding_desc& d, const void* ids, const vo
   int* order = start + d.vocab + 1;
   embed_sort_kernel<<<dim3((unsigned)((d.vocab + kBins - 1) / kBins)), dim3(kSortWaves * 64), 0, stream>>>(
       ids, d.id_bits, d.rows, d.vocab, d.padding_idx, start, order);
-  const hipError_t e = hipGetLastError();
+  hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
-  embed_sum_kernel<T><<<dim3((unsigned)((d.vocab + 3) / 4)), dim3(256), 0, stream>>>(
-      start, order, static_cast<const T*>(grad), d.grad_stride, d.dim, d.vocab, d.scale, grad_weight,
-      d.grad_weight_dtype == WFE_F32);
+  SumArgs p{};
+  p.start = start;
+  p.order = order;
+  p.ids = ids;
+  p.id_bits = d.id_bits;
+  p.grad = grad;
+  p.ld = d.grad_stride;
+  p.rows = d.rows;
+  p.dim = d.dim;
+  p.vocab = d.vocab;
+  p.scale = d.scale;
+  p.out = grad_weight;
+  p.out_f32 = d.grad_weight_dtype == WFE_F32;
+  p.partial = reinterpret_cast<float*>(static_cast<char*>(workspace) + index_bytes(d));
+  // no row can be heavy with kPiece tokens or fewer
+  const int64_t slabs = (d.dim + 64 * Vec<T>::kN - 1) / (64 * Vec<T>::kN);
+  const int64_t pieces = d.rows > kPiece ? (d.rows + kPiece - 1) / kPiece : 0;
+  const int64_t piece_blocks = (pieces * slabs + 3) / 4;
+  const int64_t row_blocks = (d.vocab + 4 * kRowsPerWave - 1) / (4 * kRowsPerWave);
+  embed_sum_kernel<T><<<dim3((unsigned)(piece_blocks + row_blocks)), dim3(256), 0, stream>>>(p, (int)piece_blocks);
+  e = hipGetLastError();
+  if (e != hipSuccess || pieces == 0) return e;
+  embed_join_kernel<T><<<dim3((unsigned)(pieces * slabs)), dim3(kJoinWaves * 64), 0, stream>>>(p);
   return hipGetLastError();
 }
 
 }  // namespace
 
-int64_t embedding_workspace_bytes(const wfe_embedding_desc& d) { return 4 * ((int64_t)d.vocab + 1 + d.rows); }
+int64_t embedding_workspace_bytes(const wfe_embedding_desc& d) {
+  return index_bytes(d) + (d.rows > kPiece ? (d.rows + kPiece - 1) / kPiece * 2 * (int64_t)d.dim * 4 : 0);
+}
 
 hipError_t launch_embedding(const wfe_embedding_desc& d, const void* ids, const void* weight, void* out,
                             hipStream_t stream) {

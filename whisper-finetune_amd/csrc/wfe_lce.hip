@@ -439,7 +439,10 @@ __device__ inline void copy_row(const T* in, T* out, int dim, int dim_pad, int l
 }
 
 // Block b takes rows [b per_block, ...): the kept rows before it are counted again by every block (a read of at most
-// all labels, out of L2), which saves a pass and its launch.
+// all labels, out of L2), which saves a pass and its launch.  Rows behind the last kept one stay as they are: they
+// reach only sums that nobody reads.
+constexpr int kPackRows = 16;
+
 template <typename T>
 __global__ __launch_bounds__(256) void lce_pack_kernel(const PackArgs p) {
   __shared__ int counts[4];
@@ -453,7 +456,6 @@ __global__ __launch_bounds__(256) void lce_pack_kernel(const PackArgs p) {
   if (lane == 0) counts[wave] = before;
   __syncthreads();
   int at = counts[0] + counts[1] + counts[2] + counts[3];
-  if (blockIdx.x == 0 && threadIdx.x == 0) p.st.head[1] = 0;
   for (long long n0 = first; n0 < last; n0 += 64) {
     __syncthreads();
     if (wave == 0) {
@@ -475,7 +477,7 @@ __global__ __launch_bounds__(256) void lce_pack_kernel(const PackArgs p) {
     }
     __syncthreads();
     at += counts[0];
-    for (int i = wave; i < 64; i += 4) {
+    for (int i = wave; i < min(64ll, last - n0); i += 4) {
       const int r = slot_of[i];
       if (r < 0) continue;
       const long long n = n0 + i;
@@ -483,13 +485,7 @@ __global__ __launch_bounds__(256) void lce_pack_kernel(const PackArgs p) {
       copy_row<T>(in, static_cast<T*>(p.packed) + (long long)r * p.dim_pad, p.dim, p.dim_pad, lane, 64, 1.f, false);
     }
   }
-  if (blockIdx.x == gridDim.x - 1) {                     // knows the number of kept rows; zeros to the next whole tile
-    if (threadIdx.x == 0) p.st.head[0] = at;
-    const long long end = ((long long)at + kLceRowPad - 1) / kLceRowPad * kLceRowPad;
-    for (long long r = at + wave; r < end; r += 4)
-      copy_row<T>(static_cast<const T*>(p.hidden), static_cast<T*>(p.packed) + r * p.dim_pad, 0, p.dim_pad, lane, 64,
-                  1.f, false);
-  }
+  if (blockIdx.x == gridDim.x - 1 && threadIdx.x == 0) p.st.head[0] = at;      // the number of kept rows
 }
 
 // The backward pass packs again from the index the forward pass left: plain rows for PROB, and for a loss that is
@@ -525,12 +521,13 @@ template <typename T>
 __global__ __launch_bounds__(256) void lce_repack_kernel(const RepackArgs p) {
   const int count = p.st.head[0];
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  const long long end = ((long long)count + kLceRowPad - 1) / kLceRowPad * kLceRowPad;
-  const long long r0 = (long long)blockIdx.x * 64;
+  // DWEI goes over the rows in whole K tiles: zeros up to there
+  const long long end = ((long long)count + kKElems<T> - 1) / kKElems<T> * kKElems<T>;
+  const long long r0 = (long long)blockIdx.x * kPackRows;
   if (r0 >= end && blockIdx.x > 0) return;
   const float shared = p.per_row ? *p.factor : p.mean ? p.upstream[0] / (float)count : p.upstream[0];
   if (!p.per_row && blockIdx.x == 0 && threadIdx.x == 0) *p.factor = shared;
-  for (long long r = r0 + wave; r < min(r0 + 64, end); r += 4) {
+  for (long long r = r0 + wave; r < min(r0 + kPackRows, end); r += 4) {
     const bool kept = r < count;
     const long long n = kept ? p.st.index[r] : 0;
     const T* in = static_cast<const T*>(p.hidden) + (n / p.inner) * p.outer_stride + (n % p.inner) * p.inner_stride;
@@ -554,57 +551,56 @@ __global__ __launch_bounds__(256) void lce_pad_weight_kernel(const T* weight, lo
 }
 
 // ---- losses out of the tiles' statistics --------------------------------------------------------------------
-// 16 rows per block, 16 threads per row over the vocabulary tiles; the block that ends last adds the rows' losses up,
-// in float64 and in a fixed order.
+// 16 rows per block, 16 threads per row over the vocabulary tiles.
 __global__ __launch_bounds__(256) void lce_loss_kernel(const float2* partial, int tiles, long long row_pad,
-                                                       LceState st, float* losses, float* total, int mean,
-                                                       float* row_loss) {
+                                                       LceState st, float* losses, float* row_loss) {
   const int count = st.head[0];
+  if ((long long)blockIdx.x * 16 >= count) return;
   const int col = threadIdx.x & 15, part = threadIdx.x >> 4;
-  const long long r = (long long)blockIdx.x * 16 + col;
+  const int r = blockIdx.x * 16 + col;
   __shared__ float2 red[16][16];
-  __shared__ double sums[4];
-  __shared__ int is_last;
-  if ((long long)blockIdx.x * 16 < count) {
-    float top = -INFINITY, sum = 0.f;
-    if (r < count)
-      for (int t = part; t < tiles; t += 16) {
-        const float2 o = partial[(long long)t * row_pad + r];
-        const float m = fmaxf(top, o.x), ref = m == -INFINITY ? 0.f : m;
-        sum = sum * exp_of(top - ref) + o.y * exp_of(o.x - ref);
+  float top = -INFINITY, sum = 0.f;
+  if (r < count) {
+    const float2* from = partial + r;
+    for (int t0 = part; t0 < tiles; t0 += 16 * 8) {           // 8 loads in flight
+      float2 o[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        o[k] = t0 + 16 * k < tiles ? from[(long long)(t0 + 16 * k) * row_pad] : make_float2(-INFINITY, 0.f);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const float m = fmaxf(top, o[k].x), ref = m == -INFINITY ? 0.f : m;
+        sum = sum * exp_of(top - ref) + o[k].y * exp_of(o[k].x - ref);
         top = m;
       }
-    red[part][col] = make_float2(top, sum);
-    __syncthreads();
-    if (part == 0 && r < count) {
-      top = -INFINITY;
-      for (int i = 0; i < 16; ++i) top = fmaxf(top, red[i][col].x);
-      const float ref = top == -INFINITY ? 0.f : top;
-      sum = 0.f;
-      for (int i = 0; i < 16; ++i) sum += red[i][col].y * exp_of(red[i][col].x - ref);
-      const float lse = st.label[r] < 0 ? __builtin_nanf("") : top + logf(sum);
-      const float loss = lse - st.zlab[r];
-      st.lse[r] = lse;
-      row_loss[r] = loss;
-      if (losses) losses[st.index[r]] = loss;
     }
   }
-  if (!total) return;
-  __threadfence();
+  red[part][col] = make_float2(top, sum);
   __syncthreads();
-  if (threadIdx.x == 0)
-    is_last = __hip_atomic_fetch_add(&st.head[1], 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == (int)gridDim.x - 1;
-  __syncthreads();
-  if (!is_last) return;
-  __threadfence();
+  if (part > 0 || r >= count) return;
+  for (int i = 1; i < 16; ++i) top = fmaxf(top, red[i][col].x);
+  const float ref = top == -INFINITY ? 0.f : top;
+  sum = 0.f;
+  for (int i = 0; i < 16; ++i) sum += red[i][col].y * exp_of(red[i][col].x - ref);
+  const float lse = st.label[r] < 0 ? __builtin_nanf("") : top + logf(sum);
+  const float loss = lse - st.zlab[r];
+  st.lse[r] = lse;
+  row_loss[r] = loss;
+  if (losses) losses[st.index[r]] = loss;
+}
+
+// sum or mean of the kept rows' losses, in float64 and in a fixed order.  (A launch of its own: one block telling the
+// last of the others by a counter needs every block's writes out of its XCD's L2 first, which took 50 us.)
+__global__ __launch_bounds__(1024) void lce_total_kernel(const float* row_loss, LceState st, float* total, int mean) {
+  __shared__ double sums[16];
+  const int count = st.head[0];
   double s = 0.0;
-  for (int i = threadIdx.x; i < count; i += 256)
-    s += __hip_atomic_load(&row_loss[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  for (int i = threadIdx.x; i < count; i += 1024) s += row_loss[i];
   for (int d = 32; d > 0; d >>= 1) s += __shfl_xor(s, d);
   if ((threadIdx.x & 63) == 0) sums[threadIdx.x >> 6] = s;
   __syncthreads();
   if (threadIdx.x == 0) {
-    s = sums[0] + sums[1] + sums[2] + sums[3];
+    for (int i = 1; i < 16; ++i) s += sums[i];
     *total = (float)(mean ? s / (double)count : s);
   }
 }
@@ -674,7 +670,12 @@ Plan make_plan(const wfe_linear_ce& d, const void* weight, bool backward, int gr
     long long piece = kPieceBytes / (p.row_pad * p.size) / kLceRowPad * kLceRowPad;
     piece = piece < kLceRowPad ? kLceRowPad : piece > all ? all : piece;
     p.piece = (int)piece;
-    p.splits = 4;
+    // DHID has few tiles of its own: its K, the vocabulary, is split until there are two blocks for each of the 256 CUs,
+    // each with at least 8 K tiles
+    const long long tiles = up(p.dim_pad, kBA) / kBA * (up(d.rows > 0 ? d.rows : 1, kBB) / kBB);
+    long long splits = (512 + tiles - 1) / tiles;
+    const long long most = (p.piece / p.ke + 7) / 8;
+    p.splits = (int)(splits > most ? most : splits);
     if (grads & WFE_GRAD_WEIGHT) {
       if (d.reduction == WFE_REDUCE_NONE) p.weighted = take(p.row_pad * p.dim_pad * p.size);
     }
@@ -744,7 +745,7 @@ hipError_t forward(const wfe_linear_ce& d, const void* hidden, const void* weigh
   k.dim = d.dim;
   k.dim_pad = p.dim_pad;
   k.vocab = d.vocab;
-  k.per_block = (int)(d.rows <= 64 * 1024 ? 64 : up((d.rows + 1023) / 1024, 64));
+  k.per_block = (int)(d.rows <= kPackRows * 1024 ? kPackRows : up((d.rows + 1023) / 1024, 64));
   k.hidden = hidden;
   k.packed = ws + p.packed;
   k.st = st;
@@ -759,9 +760,13 @@ hipError_t forward(const wfe_linear_ce& d, const void* hidden, const void* weigh
   a.a_tiles = (d.vocab + kBA - 1) / kBA;
   a.b_tiles = (int)((d.rows + kBB - 1) / kBB);
   if (d.rows > 0) LCE_TRY((launch_tiles<T, kStats>(a, (long long)a.a_tiles * a.b_tiles, stream)));
-  lce_loss_kernel<<<dim3((unsigned)(d.rows > 0 ? (d.rows + 15) / 16 : 1)), dim3(256), 0, stream>>>(
-      a.partial, a.a_tiles, p.row_pad, st, none ? loss : nullptr, none ? nullptr : loss,
-      d.reduction == WFE_REDUCE_MEAN, reinterpret_cast<float*>(ws + p.row_loss));
+  float* row_loss = reinterpret_cast<float*>(ws + p.row_loss);
+  if (d.rows > 0) {
+    lce_loss_kernel<<<dim3((unsigned)((d.rows + 15) / 16)), dim3(256), 0, stream>>>(
+        a.partial, a.a_tiles, p.row_pad, st, none ? loss : nullptr, row_loss);
+    LCE_TRY(hipGetLastError());
+  }
+  if (!none) lce_total_kernel<<<dim3(1), dim3(1024), 0, stream>>>(row_loss, st, loss, d.reduction == WFE_REDUCE_MEAN);
   return hipGetLastError();
 }
 
@@ -790,7 +795,7 @@ hipError_t backward(const wfe_linear_ce& d, const void* hidden, const void* weig
     lce_top_kernel<<<dim3(1), dim3(1024), 0, stream>>>(upstream, st, k.factor);
     LCE_TRY(hipGetLastError());
   }
-  lce_repack_kernel<T><<<dim3((unsigned)(p.row_pad / 64)), dim3(256), 0, stream>>>(k);
+  lce_repack_kernel<T><<<dim3((unsigned)(p.row_pad / kPackRows)), dim3(256), 0, stream>>>(k);
   LCE_TRY(hipGetLastError());
   if (p.copy_weight) LCE_TRY(pad_weight<T>(d, p, weight, ws, stream));
   TileArgs a{};
