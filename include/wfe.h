@@ -264,10 +264,11 @@ int64_t wfe_linear_ce_workspace_bytes(const wfe_linear_ce* d, const void* weight
 int wfe_linear_ce_forward(const wfe_linear_ce* d, const void* hidden, const void* weight, const void* labels,
                           float* loss, void* state, void* workspace, int64_t workspace_bytes, void* stream);
 /* upstream: float32 gradient of `loss` (as many entries as it).  grad_hidden (rows, dim) and grad_weight
- * (vocab, dim), contiguous, fully overwritten; either may be NULL.  hidden, weight and state as in the forward pass. */
-int wfe_linear_ce_backward(const wfe_linear_ce* d, const void* hidden, const void* weight, const void* state,
-                           const float* upstream, void* grad_hidden, void* grad_weight, void* workspace,
-                           int64_t workspace_bytes, void* stream);
+ * (vocab, dim), contiguous, fully overwritten; either may be NULL.  weight and state as in the forward pass (the
+ * state holds the rows of hidden that count). */
+int wfe_linear_ce_backward(const wfe_linear_ce* d, const void* weight, const void* state, const float* upstream,
+                           void* grad_hidden, void* grad_weight, void* workspace, int64_t workspace_bytes,
+                           void* stream);
 
 /* out_n = scale * W_{ids_n}, rounded once; a row of NaN for an id outside 0..vocab-1.  The gradient of W is
  * scale * (sum of grad_out_n over the n with ids_n = v, in float32 and in the order of n), zero for padding_idx and for

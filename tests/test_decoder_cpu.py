@@ -66,7 +66,7 @@ def test_c_linear_ce_refuses(bad):
     assert lib.wfe_linear_ce_state_bytes(C.byref(d)) == _lib.ERR_ARG
     assert lib.wfe_linear_ce_workspace_bytes(C.byref(d), None, 1, 3) == _lib.ERR_ARG
     assert lib.wfe_linear_ce_forward(C.byref(d), 64, 64, 64, 64, 64, 64, 1 << 40, None) == _lib.ERR_ARG
-    assert lib.wfe_linear_ce_backward(C.byref(d), 64, 64, 64, 64, 64, 64, 64, 1 << 40, None) == _lib.ERR_ARG
+    assert lib.wfe_linear_ce_backward(C.byref(d), 64, 64, 64, 64, 64, 64, 1 << 40, None) == _lib.ERR_ARG
     assert b"linear_ce" in lib.wfe_last_error(None)
 
 
@@ -103,10 +103,10 @@ def test_c_pointers_and_workspaces():
     assert fwd(C.byref(d), 64, 64, 64, 64, 64, 72, need, None) == _lib.ERR_ARG
     assert fwd(None, 64, 64, 64, 64, 64, 64, need, None) == _lib.ERR_ARG
     bwd = lib.wfe_linear_ce_backward
-    assert bwd(C.byref(d), 64, 64, 64, 64, None, None, None, 0, None) == 0               # nothing wanted
-    assert bwd(C.byref(d), 64, 64, 64, 64, 66, None, 64, both, None) == _lib.ERR_ARG
-    assert bwd(C.byref(d), 64, 64, None, 64, 64, None, 64, both, None) == _lib.ERR_ARG
-    assert bwd(C.byref(d), 64, 64, 64, 64, 64, 64, 64, both - 1, None) == _lib.ERR_ARG
+    assert bwd(C.byref(d), 64, 64, 64, None, None, None, 0, None) == 0               # nothing wanted
+    assert bwd(C.byref(d), 64, 64, 64, 66, None, 64, both, None) == _lib.ERR_ARG
+    assert bwd(C.byref(d), 64, None, 64, 64, None, 64, both, None) == _lib.ERR_ARG
+    assert bwd(C.byref(d), 64, 64, 64, 64, 64, 64, both - 1, None) == _lib.ERR_ARG
     e = _emb()
     need = lib.wfe_embedding_workspace_bytes(C.byref(e))
     assert lib.wfe_embedding(C.byref(e), 64, None, 64, None) == _lib.ERR_ARG

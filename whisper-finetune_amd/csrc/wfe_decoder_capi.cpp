@@ -107,7 +107,7 @@ extern "C" {
 
 int64_t wfe_linear_ce_state_bytes(const wfe_linear_ce* d) {
   CHECKED(check_ce(d));
-  return wfe::lce_state_bytes(d->rows);
+  return wfe::lce_state_bytes(*d);
 }
 
 int64_t wfe_linear_ce_workspace_bytes(const wfe_linear_ce* d, const void* weight, int32_t backward, int32_t grads) {
@@ -131,22 +131,22 @@ int wfe_linear_ce_forward(const wfe_linear_ce* d, const void* hidden, const void
                                           static_cast<hipStream_t>(stream)), "linear_ce forward");
 }
 
-int wfe_linear_ce_backward(const wfe_linear_ce* d, const void* hidden, const void* weight, const void* state,
-                           const float* upstream, void* grad_hidden, void* grad_weight, void* workspace,
-                           int64_t workspace_bytes, void* stream) {
+int wfe_linear_ce_backward(const wfe_linear_ce* d, const void* weight, const void* state, const float* upstream,
+                           void* grad_hidden, void* grad_weight, void* workspace, int64_t workspace_bytes,
+                           void* stream) {
   CHECKED(check_ce(d));
   if (!grad_hidden && !grad_weight) return WFE_OK;
-  if (!weight || !state || (d->rows > 0 && !hidden) || (!upstream && (d->rows > 0 || d->reduction)))
+  if (!weight || !state || (!upstream && (d->rows > 0 || d->reduction)))
     return wfe::fail(nullptr, WFE_ERR_ARG, "linear_ce: null device pointer");
-  if (!aligned(state, 16) || !aligned(upstream, 4) || !aligned(hidden, size_of(d->dtype)) ||
-      !aligned(weight, size_of(d->dtype)) || !aligned(grad_hidden, 16) || !aligned(grad_weight, 16))
+  if (!aligned(state, 16) || !aligned(upstream, 4) || !aligned(weight, size_of(d->dtype)) ||
+      !aligned(grad_hidden, 16) || !aligned(grad_weight, 16))
     return wfe::fail(nullptr, WFE_ERR_ARG, "linear_ce: misaligned pointer (gradients start on 16 bytes)");
   const int grads = (grad_hidden ? WFE_GRAD_HIDDEN : 0) | (grad_weight ? WFE_GRAD_WEIGHT : 0);
   CHECKED(check_workspace(workspace, workspace_bytes, wfe::lce_workspace_bytes(*d, weight, 1, grads), "linear_ce"));
   CHECKED(check_device(d->device));
   wfe::DeviceGuard guard(d->device);
   if (!guard.ok) return wfe::fail(nullptr, WFE_ERR_HIP, "hipSetDevice(%d) failed", d->device);
-  return launched(wfe::launch_lce_backward(*d, hidden, weight, state, upstream, grad_hidden, grad_weight, workspace,
+  return launched(wfe::launch_lce_backward(*d, weight, state, upstream, grad_hidden, grad_weight, workspace,
                                            static_cast<hipStream_t>(stream)), "linear_ce backward");
 }
 

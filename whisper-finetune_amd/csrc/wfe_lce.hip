@@ -4,9 +4,9 @@
 //   d[n][v] = exp(z[n][v] - lse_n) - [v == y_n]
 //   dh_n = g_n sum_v d[n][v] W_v          dW_v = sum_n g_n d[n][v] h_n          (g_n: upstream share of row n)
 //
-// Rows whose label is ignore_index are dropped first: lce_pack_kernel copies the kept ones together (and pads
-// them with zeros to whole tiles), every product after it runs over the kept rows only, whose number stays on the
-// device.  All four products are one tile kernel that multiplies 16-byte K fragments out of LDS:
+// Rows whose label is ignore_index are dropped first: lce_pack_kernel copies the kept ones together, every product
+// after it runs over the kept rows only, whose number stays on the device.  All four products are one tile routine that
+// multiplies 16-byte K fragments out of LDS:
 //   STATS  z tiles, reduced in registers to a maximum and a sum of exponentials per row and vocabulary tile
 //   PROB   z tiles again, written as d for a piece of the vocabulary
 //   DHID   dh += d W over that piece, in float32
@@ -61,24 +61,26 @@ template <> struct Elem<float> {
   static constexpr float kScale = 1.0f;
 };
 
-constexpr int kKBytes = 128;                               // depth of a K tile in bytes
+constexpr int kKBytes = 64;                                // depth of a K tile in bytes: one MFMA step of 2-byte types
+constexpr int kPadBytes = 128;                             // packed rows are whole multiples of this
+constexpr int kPadRows = 64;                               // zeros follow the kept rows up to a multiple of this
 template <typename T> constexpr int kKElems = kKBytes / (int)sizeof(T);
 constexpr float kLog2e = 1.44269504088896340736f;
 
 __device__ inline float exp_of(float x) { return __builtin_amdgcn_exp2f(x * kLog2e); }
 
 // ---- operands -------------------------------------------------------------------------------------------
-// An operand tile in LDS is either a rows x 128 bytes of K ("along": K contiguous in memory) or K rows x columns
+// An operand tile in LDS is either rows x 64 bytes of K ("along": K contiguous in memory) or K rows x columns
 // ("across": K strided in memory, transposed by the read).  16-byte chunks of a row are permuted by an exclusive or
 // so that the lanes of a fragment read meet different banks:
-//   along           chunk ^ (row & 7)
+//   along           rows of 4 chunks, 4 rows cover the banks: the rows 4 apart take different chunks
 //   across, 2 byte  pairs of chunks (a transposing read takes 32 bytes of each of 4 rows); 8 rows 0..3, 8..11 apart
 //   across, 4 byte  groups of four chunks; 4 rows 4 apart
-template <typename T, bool ACROSS>
+template <typename T, bool ACROSS, int N>
 __device__ inline int swizzle(int row) {
-  if constexpr (!ACROSS) return row & 7;
-  else if constexpr (sizeof(T) == 2) return ((row & 3) | ((row >> 1) & 4)) << 1;
-  else return ((row >> 2) & 3) << 2;
+  if constexpr (!ACROSS) return (row >> 2) & 3;
+  else if constexpr (sizeof(T) == 2) return (((row & 3) | ((row >> 1) & 4)) & (N / 16 - 1)) << 1;
+  else return (((row >> 2) & 3) & (N / 16 - 1)) << 2;
 }
 
 // Loads tiles of N rows (or columns) with NW waves, 1024 bytes per wave and instruction straight into LDS.
@@ -114,9 +116,9 @@ struct Loader {
     }
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
-      const int id = (i * NW + wave) * 64 + lane;
+      const int id = (i * NW + wave) % kInstrs * 64 + lane;     // (a small tile: some waves fetch the same again)
       int row = id / kChunks;
-      int c = (id % kChunks) ^ swizzle<T, ACROSS>(row);
+      int c = (id % kChunks) ^ swizzle<T, ACROSS, N>(row);
       if constexpr (ACROSS) {
         const int most = (int)((limit - first) * (int)sizeof(T) / 16) - 1;
         c = c < most ? c : most;          // columns past the end: any that exist, their products are not stored
@@ -127,17 +129,17 @@ struct Loader {
       off[i] = (unsigned)(row * ld) + (unsigned)c * 16u;
     }
   }
+  // LAST: the tile may reach past the K rows that exist; those that do not are read as the last one that does (their
+  // factors on the other side are 0)
+  template <bool LAST>
   __device__ void issue(char* lds) {
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
-      const int instr = i * NW + wave;
-      if (kInstrs % NW != 0 && instr >= kInstrs) break;
+      const int instr = (i * NW + wave) % kInstrs;
       unsigned o = off[i];
-      if constexpr (ACROSS) {
-        if (k_left < kKElems<T>) {        // K rows past the end: the last one (its factors on the other side are 0)
-          const int row = (instr * 64 + lane) / kChunks;
-          if (row >= k_left) o -= (unsigned)((row - k_left + 1) * ld);
-        }
+      if constexpr (ACROSS && LAST) {
+        const int row = (instr * 64 + lane) / kChunks;
+        o -= (unsigned)(max(row - k_left + 1, 0) * ld);
       }
       __builtin_amdgcn_global_load_lds(
           (const __attribute__((address_space(1))) void*)(base + o),
@@ -148,40 +150,55 @@ struct Loader {
   }
 };
 
-// Fragment of 16 rows (or columns) from m0 on, K step ks (0 or 1) of the tile
+// Fragment of 16 rows (or columns) from m0 on
 template <typename T, bool ACROSS, int N>
-__device__ inline Frag read_frag(const char* lds, int m0, int ks, int lane) {
+__device__ inline Frag read_frag(const char* lds, int m0, int lane) {
   Frag r;
   if constexpr (!ACROSS) {
     const int row = m0 + (lane & 15);
-    const int c = (ks * 4 + (lane >> 4)) ^ (row & 7);
+    const int c = (lane >> 4) ^ swizzle<T, false, N>(row);
     r.i = *reinterpret_cast<const i32x4*>(lds + row * kKBytes + c * 16);
   } else if constexpr (sizeof(T) == 2) {
     const int g = lane >> 4, j = (lane & 15) >> 2, q = lane & 3;
     const int chunk = m0 / 8 + (q >> 1);
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const int row = ks * 32 + 8 * g + 4 * h + j;
+      const int row = 8 * g + 4 * h + j;
       r.s[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(
-          lds + row * (N * 2) + (chunk ^ swizzle<T, true>(row)) * 16 + (q & 1) * 8));
+          lds + row * (N * 2) + (chunk ^ swizzle<T, true, N>(row)) * 16 + (q & 1) * 8));
     }
   } else {
     const int col = m0 + (lane & 15);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int row = ks * 16 + 4 * (lane >> 4) + i;
-      r.f[i] = *reinterpret_cast<const float*>(lds + row * (N * 4) + ((col / 4) ^ swizzle<T, true>(row)) * 16 +
+      const int row = 4 * (lane >> 4) + i;
+      r.f[i] = *reinterpret_cast<const float*>(lds + row * (N * 4) + ((col / 4) ^ swizzle<T, true, N>(row)) * 16 +
                                                (col & 3) * 4);
     }
   }
   return r;
 }
 
-// ---- the tile kernel ----------------------------------------------------------------------------------------
+// ---- the tile routine --------------------------------------------------------------------------------------
+template <int N> struct Const { static constexpr int value = N; };
+struct Yes { static constexpr bool value = true; };
+struct No { static constexpr bool value = false; };
 enum Mode { kStats, kProb, kDhid, kDwei };
 
+// A block's tile: BA x BB results of WA x WB waves, S K tiles in LDS, PER blocks on a CU at a time
+template <int BA_, int BB_, int WA_, int WB_, int S_, int PER_>
+struct Cfg {
+  static constexpr int BA = BA_, BB = BB_, WA = WA_, WB = WB_, S = S_, PER = PER_;
+  static constexpr int kThreads = WA * WB * 64;
+  static constexpr int kWavesPerSimd = PER * WA * WB / 4;
+  static constexpr int kSlots = 256 * PER;                 // blocks that run at once on 256 CUs
+  static constexpr int kStage = (BA + BB) * kKBytes;
+  static constexpr int kLds = S * kStage;
+};
+
 struct TileArgs {
-  const void* hidden;     // packed rows (row_pad, dim_pad); DWEI: the weighted ones
+  const void* hidden;     // packed rows (row_pad, dim_pad)
+  const void* weighted;   // DWEI: the same, or rows times their own weight
   const void* weight;     // (vocab, dim_pad) from row v0 on, weight_ld elements apart
   void* prob;             // d of the piece, (row_pad, prob_ld)
   long long weight_ld, prob_ld;
@@ -193,38 +210,28 @@ struct TileArgs {
   const float* lse;
   float2* partial;        // STATS: (vocabulary tiles, row_pad) maximum and sum
   float* acc;             // DHID: (splits, row_pad, dim_pad)
-  int splits, first;
+  int first;              // DHID: acc starts with this piece
   void* grad_weight;      // DWEI: (vocab, dim)
   int grad_f32;
-  const float* factor;    // DWEI
-  int a_tiles, b_tiles;   // tiles along the two axes; of rows: the most there can be
+  const float* factor;    // DWEI: multiplied with; mean: divided by the number of kept rows
+  int mean;
 };
 
-template <typename T, int MODE, int BA, int BB, int WA, int WB>
-__global__ __launch_bounds__(WA * WB * 64) void lce_tile_kernel(const TileArgs p) {
+// The id-th of `a_tiles` x `b_tiles` tiles of part `split` of `splits` of K.  smem: C::kLds bytes.
+template <typename T, class C, int MODE>
+__device__ __forceinline__ void run_tile(const TileArgs& p, int count, int id, int a_tiles, int b_tiles, int splits,
+                                         char* smem) {
   constexpr bool kAAcross = MODE == kDhid || MODE == kDwei;
   constexpr bool kBAcross = MODE == kDwei;
+  constexpr int BA = C::BA, BB = C::BB, WA = C::WA, WB = C::WB, kStages = C::S, kStage = C::kStage;
   constexpr int NW = WA * WB, TA = BA / WA, TB = BB / WB, FA = TA / 16, FB = TB / 16;
-  constexpr int kStage = (BA + BB) * kKBytes;
   constexpr int KE = kKElems<T>;
-  extern __shared__ __align__(1024) char smem[];
-
-  const int count = p.head[0];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
 
-  // Which tile: blocks go to the 8 XCDs in turn; each XCD takes a contiguous run of the tiles, ordered so that a few
-  // tiles of one axis are reused from its L2 while the other axis passes.
-  const int a_tiles = p.a_tiles;
-  const int b_tiles = MODE == kDwei ? p.b_tiles : (count + BB - 1) / BB;
   const int plane = a_tiles * b_tiles;
-  const int total = plane * (MODE == kDhid ? p.splits : 1);
-  const int per = (total + 7) / 8;
-  const int slot = blockIdx.x >> 3;
-  int id = (blockIdx.x & 7) * per + slot;
-  if (slot >= per || id >= total) return;
   const int split = id / plane;
   id -= split * plane;
-  constexpr int kGroup = 8;
+  constexpr int kGroup = 8;                                // tiles of one axis that stay in an XCD's L2 as the other passes
   const int group = id / (kGroup * a_tiles);
   const int rest = id - group * kGroup * a_tiles;
   const int in_group = min(kGroup, b_tiles - group * kGroup);
@@ -237,25 +244,23 @@ __global__ __launch_bounds__(WA * WB * 64) void lce_tile_kernel(const TileArgs p
   else if constexpr (MODE == kDwei) k_tiles = (count + KE - 1) / KE;
   else {
     const int all = (p.piece + KE - 1) / KE;
-    const int each = (all + p.splits - 1) / p.splits;
-    k_first = split * each;
+    const int each = (all + splits - 1) / splits;
+    k_first = min(split * each, all);
     k_tiles = min(each, all - k_first);
-    if (k_tiles < 0) k_tiles = 0;
   }
 
   Loader<T, kAAcross, BA, NW> la;
   Loader<T, kBAcross, BB, NW> lb;
-  const T* hidden = static_cast<const T*>(p.hidden);
   const T* weight = static_cast<const T*>(p.weight);
   const T* prob = static_cast<const T*>(p.prob);
   if constexpr (MODE == kStats || MODE == kProb) {
     la.init(weight, p.weight_ld, a0, p.piece, 0, 0, wave, lane);
-    lb.init(hidden, p.dim_pad, b0, b0 + BB, 0, 0, wave, lane);
+    lb.init(static_cast<const T*>(p.hidden), p.dim_pad, b0, b0 + BB, 0, 0, wave, lane);
   } else if constexpr (MODE == kDhid) {
     la.init(weight, p.weight_ld, a0, p.dim_pad, (long long)k_first * KE, p.piece, wave, lane);
     lb.init(prob, p.prob_ld, b0, b0 + BB, (long long)k_first * KE, 0, wave, lane);
   } else {
-    la.init(hidden, p.dim_pad, a0, p.dim_pad, 0, p.row_pad, wave, lane);
+    la.init(static_cast<const T*>(p.weighted), p.dim_pad, a0, p.dim_pad, 0, p.row_pad, wave, lane);
     lb.init(prob, p.prob_ld, b0, (int)p.prob_ld, 0, p.row_pad, wave, lane);
   }
 
@@ -266,32 +271,85 @@ __global__ __launch_bounds__(WA * WB * 64) void lce_tile_kernel(const TileArgs p
 #pragma unroll
     for (int j = 0; j < FB; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-  if (k_tiles > 0) {
-    la.issue(smem);
-    lb.issue(smem + BA * kKBytes);
-  }
-  for (int t = 0; t < k_tiles; ++t) {
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-    if (t + 1 < k_tiles) {
-      char* next = smem + ((t + 1) & 1) * kStage;
-      la.issue(next);
-      lb.issue(next + BA * kKBytes);
-    }
-    const char* sa = smem + (t & 1) * kStage;
+  // kStages K tiles in LDS, all but one of them on their way while one is multiplied.  Per tile: wait until this wave's
+  // part of the oldest has arrived (the younger ones may stay under way), one barrier -- now everybody's has, and
+  // everybody has read the tile before it, whose place the next fetch takes -- then read fragments and multiply.
+  // (The barrier is written out: __syncthreads would wait for every fetch.)
+  constexpr int kFetches = decltype(la)::kPer + decltype(lb)::kPer;      // of every wave, per tile
+  auto fetch = [&](auto last, int stage) {
+    char* to = smem + stage * kStage;
+    la.template issue<decltype(last)::value>(to);
+    lb.template issue<decltype(last)::value>(to + BA * kKBytes);
+  };
+  Frag fa[FA], fb[FB];
+  auto read = [&](int stage) {
+    const char* sa = smem + stage * kStage;
     const char* sb = sa + BA * kKBytes;
 #pragma unroll
-    for (int ks = 0; ks < 2; ++ks) {
-      Frag fa[FA], fb[FB];
+    for (int i = 0; i < FA; ++i) fa[i] = read_frag<T, kAAcross, BA>(sa, wa * TA + i * 16, lane);
 #pragma unroll
-      for (int i = 0; i < FA; ++i) fa[i] = read_frag<T, kAAcross, BA>(sa, wa * TA + i * 16, ks, lane);
+    for (int j = 0; j < FB; ++j) fb[j] = read_frag<T, kBAcross, BB>(sb, wb * TB + j * 16, lane);
+  };
+  auto multiply = [&] {
 #pragma unroll
-      for (int j = 0; j < FB; ++j) fb[j] = read_frag<T, kBAcross, BB>(sb, wb * TB + j * 16, ks, lane);
+    for (int i = 0; i < FA; ++i)
 #pragma unroll
-      for (int i = 0; i < FA; ++i)
+      for (int j = 0; j < FB; ++j) acc[i][j] = Elem<T>::mma(fa[i], fb[j], acc[i][j]);
+  };
 #pragma unroll
-        for (int j = 0; j < FB; ++j) acc[i][j] = Elem<T>::mma(fa[i], fb[j], acc[i][j]);
+  for (int t = 0; t < kStages - 1; ++t)
+    if (t < k_tiles) {
+      if (t + 1 < k_tiles) fetch(No{}, t);
+      else fetch(Yes{}, t);
     }
+  int stage = 0, free = kStages - 1;
+  auto advance = [&] {
+    free = stage;
+    stage = stage + 1 == kStages ? 0 : stage + 1;
+  };
+  if constexpr (NW == 8) {
+    // Two waves per SIMD take turns: while one reads its fragments the other multiplies, one barrier per turn, the
+    // second group half a tile behind the first.
+    if (k_tiles >= kStages - 1) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((kStages - 2) * kFetches) : "memory");
+    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    asm volatile("s_barrier" ::: "memory");
+    const bool second = wave >= 4;
+    if (second) asm volatile("s_barrier" ::: "memory");
+    auto turn = [&](auto more) {
+      read(stage);
+      if constexpr (decltype(more)::value == 2) fetch(No{}, free);
+      if constexpr (decltype(more)::value == 1) fetch(Yes{}, free);
+      if constexpr (decltype(more)::value > 0)
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((kStages - 2) * kFetches) : "memory");
+      else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+      __builtin_amdgcn_sched_barrier(0);
+      __builtin_amdgcn_s_setprio(1);
+      multiply();
+      __builtin_amdgcn_s_setprio(0);
+      __builtin_amdgcn_sched_barrier(0);
+      asm volatile("s_barrier" ::: "memory");
+      advance();
+    };
+    int t = 0;
+    for (; t + kStages < k_tiles; ++t) turn(Const<2>{});
+    for (; t + kStages - 1 < k_tiles; ++t) turn(Const<1>{});
+    for (; t < k_tiles; ++t) turn(Const<0>{});
+    if (!second) asm volatile("s_barrier" ::: "memory");
+  } else {
+    auto tile = [&](auto more) {
+      if constexpr (decltype(more)::value > 0)
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((kStages - 2) * kFetches) : "memory");
+      else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+      if constexpr (decltype(more)::value == 2) fetch(No{}, free);
+      if constexpr (decltype(more)::value == 1) fetch(Yes{}, free);
+      read(stage);
+      multiply();
+      advance();
+    };
+    int t = 0;
+    for (; t + kStages < k_tiles; ++t) tile(Const<2>{});
+    for (; t + kStages - 1 < k_tiles; ++t) tile(Const<1>{});
+    for (; t < k_tiles; ++t) tile(Const<0>{});
   }
 
   // acc[i][j][e] belongs to a = a0 + wa TA + 16 i + 4 (lane / 16) + e and b = b0 + wb TB + 16 j + lane % 16
@@ -299,20 +357,30 @@ __global__ __launch_bounds__(WA * WB * 64) void lce_tile_kernel(const TileArgs p
   if constexpr (MODE == kStats) {
     __syncthreads();                                    // the last tile has been read: LDS is free
     float2* red = reinterpret_cast<float2*>(smem);
+    const bool ragged = a0 + BA > p.vocab;
 #pragma unroll
     for (int j = 0; j < FB; ++j) {
       const int n = b_lane + j * 16;
       const int y = n < count ? p.label[n] : -1;
       float top = -INFINITY;
+      if (ragged) {
+#pragma unroll
+        for (int i = 0; i < FA; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (a_lane + i * 16 + e >= p.vocab) acc[i][j][e] = -INFINITY;
+      }
+      if (__any(y >= a0 + wa * TA && y < a0 + (wa + 1) * TA)) {      // seldom: the label is in this wave's part
+#pragma unroll
+        for (int i = 0; i < FA; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (a_lane + i * 16 + e == y) p.zlab[n] = acc[i][j][e];
+      }
 #pragma unroll
       for (int i = 0; i < FA; ++i)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int v = a_lane + i * 16 + e;
-          if (v >= p.vocab) acc[i][j][e] = -INFINITY;
-          else if (v == y) p.zlab[n] = acc[i][j][e];
-          top = fmaxf(top, acc[i][j][e]);
-        }
+        for (int e = 0; e < 4; ++e) top = fmaxf(top, acc[i][j][e]);
       top = fmaxf(top, __shfl_xor(top, 16));
       top = fmaxf(top, __shfl_xor(top, 32));
       const float ref = top == -INFINITY ? 0.f : top;
@@ -374,7 +442,7 @@ __global__ __launch_bounds__(WA * WB * 64) void lce_tile_kernel(const TileArgs p
       }
     }
   } else {
-    const float factor = count > 0 ? *p.factor * (1.f / Elem<T>::kScale) : 0.f;
+    const float factor = count > 0 ? *p.factor / (p.mean ? (float)count : 1.f) * (1.f / Elem<T>::kScale) : 0.f;
     const bool whole = (p.dim & 3) == 0;
 #pragma unroll
     for (int j = 0; j < FB; ++j) {
@@ -401,6 +469,100 @@ __global__ __launch_bounds__(WA * WB * 64) void lce_tile_kernel(const TileArgs p
         }
       }
     }
+  }
+}
+
+// Blocks go to the 8 XCDs in turn.  Block b of a run of `tiles` takes a tile such that each XCD has a contiguous part
+// of the run; -1: none.  A run takes run_blocks of the grid.
+__device__ __host__ inline int run_blocks(int tiles) { return (tiles + 7) / 8 * 8; }
+__device__ inline int tile_of(int b, int tiles) {
+  const int per = (tiles + 7) / 8, id = (b & 7) * per + (b >> 3);
+  return id < tiles ? id : -1;
+}
+
+template <typename T, class C, int MODE>
+__global__ __launch_bounds__(C::kThreads, C::kWavesPerSimd) void lce_logits_kernel(const TileArgs p) {
+  extern __shared__ __align__(1024) char smem[];
+  const int count = p.head[0];
+  const int a_tiles = (p.piece + C::BA - 1) / C::BA, b_tiles = (count + C::BB - 1) / C::BB;
+  const int tiles = a_tiles * b_tiles;
+  if ((int)blockIdx.x >= run_blocks(tiles)) return;
+  const int id = tile_of(blockIdx.x, tiles);
+  if (id >= 0) run_tile<T, C, MODE>(p, count, id, a_tiles, b_tiles, 1, smem);
+}
+
+// DHID has few tiles of its own, so its K, the vocabulary, is split.  Beside DWEI: parts of half a CU's share of all
+// the work.  Alone: the number of parts (of up to 8, or about one round) that leaves the fewest CUs idle in the last
+// round.
+struct SplitRule {
+  int dim_tiles, bb, piece_steps, dwei_tiles, ke, slots, most;
+};
+__device__ inline int dhid_splits(const SplitRule& r, int count) {
+  const int tiles = r.dim_tiles * ((count + r.bb - 1) / r.bb);
+  if (tiles == 0) return 1;
+  if (r.dwei_tiles > 0) {
+    const long long work = (long long)r.dwei_tiles * ((count + r.ke - 1) / r.ke) + (long long)tiles * r.piece_steps;
+    const long long part = max(work / (2 * r.slots), 8ll);
+    return (int)min((long long)r.most, (r.piece_steps + part - 1) / part);
+  }
+  int best = 1;
+  float left = 0.f;
+  for (int k = 1; k <= min(r.most, max(8, r.slots / tiles)); ++k) {
+    const int rounds = (tiles * k + r.slots - 1) / r.slots;
+    const float busy = (float)(tiles * k) / (float)(rounds * r.slots);
+    if (busy > left + 0.02f) {
+      left = busy;
+      best = k;
+    }
+  }
+  return best;
+}
+
+// The gradients' products over one piece, and the next piece's d, in one grid: long tiles first, so that the short
+// ones fill the CUs that run out of them.
+struct GradArgs {
+  TileArgs t;
+  SplitRule rule;
+  int dhid, dwei;
+  int next_v0, next_piece;      // 0: no next piece
+  const void* next_weight;
+  void* next_prob;
+};
+
+template <typename T, class C>
+__global__ __launch_bounds__(C::kThreads, C::kWavesPerSimd) void lce_grads_kernel(const GradArgs g) {
+  extern __shared__ __align__(1024) char smem[];
+  const int count = g.t.head[0];
+  const int row_tiles = (count + C::BB - 1) / C::BB;
+  const int dim_tiles = g.rule.dim_tiles;
+  int b = blockIdx.x;
+  if (g.dwei) {
+    const int b_tiles = (g.t.piece + C::BB - 1) / C::BB, tiles = dim_tiles * b_tiles;
+    if (b < run_blocks(tiles)) {
+      const int id = tile_of(b, tiles);
+      if (id >= 0) run_tile<T, C, kDwei>(g.t, count, id, dim_tiles, b_tiles, 1, smem);
+      return;
+    }
+    b -= run_blocks(tiles);
+  }
+  if (g.dhid) {
+    const int splits = dhid_splits(g.rule, count), tiles = dim_tiles * row_tiles * splits;
+    if (b < run_blocks(tiles)) {
+      const int id = tile_of(b, tiles);
+      if (id >= 0) run_tile<T, C, kDhid>(g.t, count, id, dim_tiles, row_tiles, splits, smem);
+      return;
+    }
+    b -= run_blocks(tiles);
+  }
+  if (g.next_piece > 0) {
+    TileArgs p = g.t;
+    p.v0 = g.next_v0;
+    p.piece = g.next_piece;
+    p.weight = g.next_weight;
+    p.prob = g.next_prob;
+    const int a_tiles = (p.piece + C::BA - 1) / C::BA, tiles = a_tiles * row_tiles;
+    const int id = b < run_blocks(tiles) ? tile_of(b, tiles) : -1;
+    if (id >= 0) run_tile<T, C, kProb>(p, count, id, a_tiles, row_tiles, 1, smem);
   }
 }
 
@@ -439,8 +601,7 @@ __device__ inline void copy_row(const T* in, T* out, int dim, int dim_pad, int l
 }
 
 // Block b takes rows [b per_block, ...): the kept rows before it are counted again by every block (a read of at most
-// all labels, out of L2), which saves a pass and its launch.  Rows behind the last kept one stay as they are: they
-// reach only sums that nobody reads.
+// all labels, out of L2), which saves a pass and its launch.
 constexpr int kPackRows = 16;
 
 template <typename T>
@@ -485,22 +646,15 @@ __global__ __launch_bounds__(256) void lce_pack_kernel(const PackArgs p) {
       copy_row<T>(in, static_cast<T*>(p.packed) + (long long)r * p.dim_pad, p.dim, p.dim_pad, lane, 64, 1.f, false);
     }
   }
-  if (blockIdx.x == gridDim.x - 1 && threadIdx.x == 0) p.st.head[0] = at;      // the number of kept rows
+  if (blockIdx.x == gridDim.x - 1) {         // knows the number of kept rows
+    if (threadIdx.x == 0) p.st.head[0] = at;
+    // DWEI goes over the rows in whole K tiles: zeros up to there (rows further on reach only sums that nobody reads)
+    const long long end = ((long long)at + kPadRows - 1) / kPadRows * kPadRows;
+    const long long vecs = (end - at) * p.dim_pad * (long long)sizeof(T) / 16;
+    f32x4* out = reinterpret_cast<f32x4*>(static_cast<T*>(p.packed) + (long long)at * p.dim_pad);
+    for (long long i = threadIdx.x; i < vecs; i += 256) out[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
 }
-
-// The backward pass packs again from the index the forward pass left: plain rows for PROB, and for a loss that is
-// weighted row by row (upstream of WFE_REDUCE_NONE) rows times g_n / max |g| for DWEI.
-struct RepackArgs {
-  const void* hidden;
-  long long inner, outer_stride, inner_stride;
-  int dim, dim_pad, mean, per_row;
-  LceState st;
-  const float* upstream;
-  float* row_factor;      // g of kept row r
-  float* factor;          // what DWEI multiplies with; per_row: max |g|, left by lce_top_kernel
-  void* packed;
-  void* weighted;         // null unless per_row
-};
 
 // max |g| over the kept rows
 __global__ __launch_bounds__(1024) void lce_top_kernel(const float* upstream, LceState st, float* factor) {
@@ -517,28 +671,18 @@ __global__ __launch_bounds__(1024) void lce_top_kernel(const float* upstream, Lc
   }
 }
 
+// A loss weighted row by row (upstream of WFE_REDUCE_NONE): rows times g_n / max |g| for DWEI, rounded to their type
+// once more; within [-1, 1] times the row, so that half precision neither overflows nor loses small weights first.
 template <typename T>
-__global__ __launch_bounds__(256) void lce_repack_kernel(const RepackArgs p) {
-  const int count = p.st.head[0];
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  // DWEI goes over the rows in whole K tiles: zeros up to there
-  const long long end = ((long long)count + kKElems<T> - 1) / kKElems<T> * kKElems<T>;
-  const long long r0 = (long long)blockIdx.x * kPackRows;
-  if (r0 >= end && blockIdx.x > 0) return;
-  const float shared = p.per_row ? *p.factor : p.mean ? p.upstream[0] / (float)count : p.upstream[0];
-  if (!p.per_row && blockIdx.x == 0 && threadIdx.x == 0) *p.factor = shared;
-  for (long long r = r0 + wave; r < min(r0 + kPackRows, end); r += 4) {
-    const bool kept = r < count;
-    const long long n = kept ? p.st.index[r] : 0;
-    const T* in = static_cast<const T*>(p.hidden) + (n / p.inner) * p.outer_stride + (n % p.inner) * p.inner_stride;
-    const int dim = kept ? p.dim : 0;
-    const float g = !kept ? 0.f : p.per_row ? p.upstream[n] : shared;
-    if (kept && lane == 0) p.row_factor[r] = g;
-    copy_row<T>(in, static_cast<T*>(p.packed) + r * p.dim_pad, dim, p.dim_pad, lane, 64, 1.f, false);
-    if (p.per_row && p.weighted)
-      copy_row<T>(in, static_cast<T*>(p.weighted) + r * p.dim_pad, dim, p.dim_pad, lane, 64,
-                  shared > 0.f ? g / shared : g, true);
-  }
+__global__ __launch_bounds__(256) void lce_weigh_kernel(const void* packed, void* weighted, int dim_pad, LceState st,
+                                                        const float* upstream, const float* top) {
+  const int count = st.head[0];
+  const long long r = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (r >= (count + kPadRows - 1) / kPadRows * kPadRows) return;
+  const bool kept = r < count;
+  const float g = kept ? upstream[st.index[r]] : 0.f;
+  copy_row<T>(static_cast<const T*>(packed) + r * dim_pad, static_cast<T*>(weighted) + r * dim_pad,
+              kept ? dim_pad : 0, dim_pad, threadIdx.x & 63, 64, *top > 0.f ? g / *top : g, true);
 }
 
 // W with rows that the tiles cannot read in place (odd sizes, strides or alignment): one padded copy
@@ -551,49 +695,18 @@ __global__ __launch_bounds__(256) void lce_pad_weight_kernel(const T* weight, lo
 }
 
 // ---- losses out of the tiles' statistics --------------------------------------------------------------------
-// 16 rows per block, 16 threads per row over the vocabulary tiles.
-__global__ __launch_bounds__(256) void lce_loss_kernel(const float2* partial, int tiles, long long row_pad,
-                                                       LceState st, float* losses, float* row_loss) {
-  const int count = st.head[0];
-  if ((long long)blockIdx.x * 16 >= count) return;
-  const int col = threadIdx.x & 15, part = threadIdx.x >> 4;
-  const int r = blockIdx.x * 16 + col;
-  __shared__ float2 red[16][16];
-  float top = -INFINITY, sum = 0.f;
-  if (r < count) {
-    const float2* from = partial + r;
-    for (int t0 = part; t0 < tiles; t0 += 16 * 8) {           // 8 loads in flight
-      float2 o[8];
-#pragma unroll
-      for (int k = 0; k < 8; ++k)
-        o[k] = t0 + 16 * k < tiles ? from[(long long)(t0 + 16 * k) * row_pad] : make_float2(-INFINITY, 0.f);
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const float m = fmaxf(top, o[k].x), ref = m == -INFINITY ? 0.f : m;
-        sum = sum * exp_of(top - ref) + o[k].y * exp_of(o[k].x - ref);
-        top = m;
-      }
-    }
-  }
-  red[part][col] = make_float2(top, sum);
-  __syncthreads();
-  if (part > 0 || r >= count) return;
-  for (int i = 1; i < 16; ++i) top = fmaxf(top, red[i][col].x);
-  const float ref = top == -INFINITY ? 0.f : top;
-  sum = 0.f;
-  for (int i = 0; i < 16; ++i) sum += red[i][col].y * exp_of(red[i][col].x - ref);
-  const float lse = st.label[r] < 0 ? __builtin_nanf("") : top + logf(sum);
-  const float loss = lse - st.zlab[r];
-  st.lse[r] = lse;
-  row_loss[r] = loss;
-  if (losses) losses[st.index[r]] = loss;
+// 16 rows per block and step, 64 threads per row over the vocabulary tiles.  A grid of one block takes all rows and adds
+// their losses up as well (total != null).
+constexpr int kLossParts = 64, kLossSteps = 4;
+
+__device__ inline void merge(float& top, float& sum, float2 o) {
+  const float m = fmaxf(top, o.x), ref = m == -INFINITY ? 0.f : m;
+  sum = sum * exp_of(top - ref) + o.y * exp_of(o.x - ref);
+  top = m;
 }
 
-// sum or mean of the kept rows' losses, in float64 and in a fixed order.  (A launch of its own: one block telling the
-// last of the others by a counter needs every block's writes out of its XCD's L2 first, which took 50 us.)
-__global__ __launch_bounds__(1024) void lce_total_kernel(const float* row_loss, LceState st, float* total, int mean) {
+__device__ inline void sum_losses(const float* row_loss, int count, float* total, int mean) {
   __shared__ double sums[16];
-  const int count = st.head[0];
   double s = 0.0;
   for (int i = threadIdx.x; i < count; i += 1024) s += row_loss[i];
   for (int d = 32; d > 0; d >>= 1) s += __shfl_xor(s, d);
@@ -605,52 +718,131 @@ __global__ __launch_bounds__(1024) void lce_total_kernel(const float* row_loss, 
   }
 }
 
-// dh: the splits' sums, times g, to every row's place; zeros for ignored rows
+__global__ __launch_bounds__(1024) void lce_loss_kernel(const float2* partial, int tiles, long long row_pad,
+                                                        LceState st, float* losses, float* row_loss, float* total,
+                                                        int mean) {
+  const int count = st.head[0];
+  const int col = threadIdx.x & 15, part = threadIdx.x >> 4;
+  __shared__ float2 red[kLossParts][16];
+  for (int r0 = blockIdx.x * 16; r0 < count; r0 += gridDim.x * 16) {
+    const int r = r0 + col;
+    float top = -INFINITY, sum = 0.f;
+    if (r < count) {
+      const float2* from = partial + r;
+      for (int t0 = part; t0 < tiles; t0 += kLossParts * kLossSteps) {
+        float2 o[kLossSteps];
+#pragma unroll
+        for (int k = 0; k < kLossSteps; ++k)
+          o[k] = t0 + kLossParts * k < tiles ? from[(long long)(t0 + kLossParts * k) * row_pad]
+                                             : make_float2(-INFINITY, 0.f);
+#pragma unroll
+        for (int k = 0; k < kLossSteps; ++k) merge(top, sum, o[k]);
+      }
+      // the 4 threads of this row in the wave
+      for (int d = 16; d < 64; d <<= 1) merge(top, sum, make_float2(__shfl_xor(top, d), __shfl_xor(sum, d)));
+    }
+    red[part][col] = make_float2(top, sum);
+    __syncthreads();
+    if (part == 0 && r < count) {
+      for (int i = 4; i < kLossParts; i += 4) merge(top, sum, red[i][col]);
+      const float lse = st.label[r] < 0 ? __builtin_nanf("") : top + logf(sum);
+      const float loss = lse - st.zlab[r];
+      st.lse[r] = lse;
+      row_loss[r] = loss;
+      if (losses) losses[st.index[r]] = loss;
+    }
+    __syncthreads();
+  }
+  if (total) sum_losses(row_loss, count, total, mean);
+}
+
+// sum or mean of the kept rows' losses, in float64 and in a fixed order.  (A launch of its own: one block telling the
+// last of the others by a counter needs every block's writes out of its XCD's L2 first, which took 50 us.)
+__global__ __launch_bounds__(1024) void lce_total_kernel(const float* row_loss, LceState st, float* total, int mean) {
+  sum_losses(row_loss, st.head[0], total, mean);
+}
+
+// dh: the splits' sums, times g, to every row's place; zeros for ignored rows.  One wave per row.
+struct DhidArgs {
+  const float* acc;
+  SplitRule rule;
+  long long row_pad, rows;
+  int dim, dim_pad;
+  LceState st;
+  const float* upstream;
+  int reduction, out_f32;
+  void* out;
+};
+
 template <typename T>
-__global__ __launch_bounds__(256) void lce_dhid_kernel(const float* acc, int splits, long long row_pad, int dim,
-                                                       int dim_pad, long long rows, LceState st,
-                                                       const float* row_factor, void* out, int out_f32) {
+__global__ __launch_bounds__(256) void lce_dhid_kernel(const DhidArgs p) {
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
   const long long n = (long long)blockIdx.x * 4 + wave;
-  if (n >= rows) return;
-  const int r = st.slot[n];
+  if (n >= p.rows) return;
+  const int r = p.st.slot[n], count = p.st.head[0];
   const bool kept = r >= 0;
-  const float g = kept ? row_factor[r] * (1.f / Elem<T>::kScale) : 0.f;
-  for (int d = lane * 4; d < dim; d += 256) {
+  const int splits = kept ? dhid_splits(p.rule, count) : 0;
+  float g = 0.f;
+  if (kept) {
+    g = p.upstream[p.reduction == WFE_REDUCE_NONE ? n : 0];
+    if (p.reduction == WFE_REDUCE_MEAN) g /= (float)count;
+    g *= 1.f / Elem<T>::kScale;
+  }
+  const bool whole = (p.dim & 3) == 0;
+  for (int d = lane * 4; d < p.dim; d += 256) {
     f32x4 s = {0.f, 0.f, 0.f, 0.f};
-    if (kept) {
-      for (int i = 0; i < splits; ++i)
-        s += *reinterpret_cast<const f32x4*>(acc + ((long long)i * row_pad + r) * dim_pad + d);
-      s *= g;
-    }
-    for (int e = 0; e < 4 && d + e < dim; ++e) {
-      if (out_f32) static_cast<float*>(out)[n * dim + d + e] = s[e];
-      else static_cast<T*>(out)[n * dim + d + e] = static_cast<T>(s[e]);
+    const float* from = p.acc + (long long)r * p.dim_pad + d;
+    for (int i = 0; i < splits; ++i) s += *reinterpret_cast<const f32x4*>(from + (long long)i * p.row_pad * p.dim_pad);
+    if (kept) s *= g;
+    const long long at = n * p.dim + d;
+    if (p.out_f32) {
+      float* out = static_cast<float*>(p.out) + at;
+      if (whole) *reinterpret_cast<f32x4*>(out) = s;
+      else
+        for (int e = 0; e < 4 && d + e < p.dim; ++e) out[e] = s[e];
+    } else {
+      T* out = static_cast<T*>(p.out) + at;
+      T x[4];
+      for (int e = 0; e < 4; ++e) x[e] = static_cast<T>(s[e]);
+      if (whole) __builtin_memcpy(__builtin_assume_aligned(out, 4 * sizeof(T)), x, sizeof x);
+      else
+        for (int e = 0; e < 4 && d + e < p.dim; ++e) out[e] = x[e];
     }
   }
 }
 
 // ---- host side ----------------------------------------------------------------------------------------------
-constexpr int kBA = 128, kBB = 128, kWA = 2, kWB = 2;
-constexpr long long kPieceBytes = 256ll << 20;     // most that the piece of d held at a time takes
+#ifndef WFE_L
+#define WFE_L 256, 256, 4, 2, 4, 1
+#define WFE_M 256, 128, 2, 2, 3, 2
+#define WFE_S 128, 32, 4, 1, 4, 4
+#define WFE_LROWS 768
+#endif
+using Large = Cfg<WFE_L>;
+using Medium = Cfg<WFE_M>;
+using Small = Cfg<WFE_S>;
+constexpr long long kPieceBytes = 128ll << 20;     // most that the d of one piece takes; two pieces are held
+
+long long up(long long x, long long to) { return (x + to - 1) / to * to; }
 
 struct Plan {
   int size, ke, dim_pad;
   long long row_pad;
   bool copy_weight;
-  int piece, splits;
+  int piece, pieces, splits;
   // offsets into the workspace
-  long long packed, weighted, weight, partial, row_loss, prob, acc, row_factor, factor, bytes;
+  long long weighted, weight, partial, row_loss, prob[2], acc, top, bytes;
 };
 
-long long up(long long x, long long to) { return (x + to - 1) / to * to; }
+template <class C>
+int tiles_of(long long x, bool a) { return (int)((x + (a ? C::BA : C::BB) - 1) / (a ? C::BA : C::BB)); }
 
 Plan make_plan(const wfe_linear_ce& d, const void* weight, bool backward, int grads) {
   Plan p{};
   p.size = d.dtype == WFE_F32 ? 4 : 2;
   p.ke = kKBytes / p.size;
-  p.dim_pad = (int)up(d.dim, p.ke);
-  p.row_pad = up(d.rows > 0 ? d.rows : 1, kLceRowPad);
+  p.dim_pad = lce_dim_pad(d);
+  p.row_pad = lce_row_pad(d);
   // in place: whole K tiles, 16-byte rows, offsets inside a tile in 32 bits
   p.copy_weight = !(d.dim == p.dim_pad && (d.weight_stride * p.size) % 16 == 0 &&
                     d.weight_stride * p.size < (1ll << 22) && (reinterpret_cast<uintptr_t>(weight) & 15) == 0);
@@ -660,43 +852,53 @@ Plan make_plan(const wfe_linear_ce& d, const void* weight, bool backward, int gr
     at += up(bytes, 256);
     return o;
   };
-  p.packed = take(p.row_pad * p.dim_pad * p.size);
   if (p.copy_weight) p.weight = take((long long)d.vocab * p.dim_pad * p.size);
   if (!backward) {
-    p.partial = take(up(d.vocab, kBA) / kBA * p.row_pad * 8);
+    p.partial = take(up(d.vocab, Small::BA) / Small::BA * p.row_pad * 8);
     p.row_loss = take(p.row_pad * 4);
   } else {
     const long long all = up(d.vocab, kLceRowPad);
     long long piece = kPieceBytes / (p.row_pad * p.size) / kLceRowPad * kLceRowPad;
-    piece = piece < kLceRowPad ? kLceRowPad : piece > all ? all : piece;
-    p.piece = (int)piece;
-    // DHID has few tiles of its own: its K, the vocabulary, is split until there are two blocks for each of the 256 CUs,
-    // each with at least 8 K tiles
-    const long long tiles = up(p.dim_pad, kBA) / kBA * (up(d.rows > 0 ? d.rows : 1, kBB) / kBB);
-    long long splits = (512 + tiles - 1) / tiles;
-    const long long most = (p.piece / p.ke + 7) / 8;
-    p.splits = (int)(splits > most ? most : splits);
-    if (grads & WFE_GRAD_WEIGHT) {
-      if (d.reduction == WFE_REDUCE_NONE) p.weighted = take(p.row_pad * p.dim_pad * p.size);
+    piece = piece < kLceRowPad ? kLceRowPad : piece;
+    p.pieces = (int)((all + piece - 1) / piece);
+    p.piece = (int)up((all + p.pieces - 1) / p.pieces, kLceRowPad);      // pieces of one size
+    p.pieces = (int)((all + p.piece - 1) / p.piece);
+    if ((grads & WFE_GRAD_WEIGHT) && d.reduction == WFE_REDUCE_NONE) {
+      p.weighted = take(p.row_pad * p.dim_pad * p.size);
+      p.top = take(4);
     }
-    p.prob = take(p.row_pad * p.piece * p.size);
-    if (grads & WFE_GRAD_HIDDEN) p.acc = take(p.splits * p.row_pad * p.dim_pad * 4);
-    p.row_factor = take(p.row_pad * 4);
-    p.factor = take(4);
+    p.prob[0] = take(p.row_pad * p.piece * p.size);
+    p.prob[1] = p.pieces > 1 ? take(p.row_pad * p.piece * p.size) : p.prob[0];
+    if (grads & WFE_GRAD_HIDDEN) {
+      const long long one = p.row_pad * p.dim_pad * 4;
+      const long long most = (64ll << 20) / one;           // partial sums of dh: 64 MB, or 4 parts
+      p.splits = (int)(most < 4 ? 4 : most > 64 ? 64 : most);
+      p.acc = take(p.splits * one);
+    }
   }
   p.bytes = at;
   return p;
 }
 
-template <typename T, int MODE>
-hipError_t launch_tiles(const TileArgs& a, long long tiles, hipStream_t stream) {
-  constexpr int kLds = 2 * (kBA + kBB) * kKBytes;
-  auto* kernel = lce_tile_kernel<T, MODE, kBA, kBB, kWA, kWB>;
-  const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
-                                           hipFuncAttributeMaxDynamicSharedMemorySize, kLds);
-  if (e != hipSuccess) return e;
-  if (tiles > 0x7ffffff0ll) return hipErrorInvalidValue;
-  kernel<<<dim3((unsigned)up(tiles, 8)), dim3(kWA * kWB * 64), kLds, stream>>>(a);
+#define LCE_TRY(expr)                      \
+  do {                                     \
+    const hipError_t e_ = (expr);          \
+    if (e_ != hipSuccess) return e_;       \
+  } while (0)
+
+template <auto KERNEL, class C, class A>
+hipError_t launch(const A& args, long long blocks, hipStream_t stream) {
+  static unsigned long long done = 0;           // a bit per device: more than 64 KB of LDS has been asked for
+  int device = 0;
+  LCE_TRY(hipGetDevice(&device));
+  const unsigned long long bit = 1ull << (device & 63);
+  if (!(__atomic_load_n(&done, __ATOMIC_RELAXED) & bit)) {
+    LCE_TRY(hipFuncSetAttribute(reinterpret_cast<const void*>(KERNEL), hipFuncAttributeMaxDynamicSharedMemorySize,
+                                C::kLds));
+    __atomic_fetch_or(&done, bit, __ATOMIC_RELAXED);
+  }
+  if (blocks > 0x7ffffff0ll) return hipErrorInvalidValue;
+  KERNEL<<<dim3((unsigned)blocks), dim3(C::kThreads), C::kLds, stream>>>(args);
   return hipGetLastError();
 }
 
@@ -707,33 +909,36 @@ hipError_t pad_weight(const wfe_linear_ce& d, const Plan& p, const void* weight,
   return hipGetLastError();
 }
 
-void fill_tiles(TileArgs& a, const wfe_linear_ce& d, const Plan& p, const void* weight, char* ws, const LceState& st) {
-  a.hidden = ws + p.packed;
+TileArgs tile_args(const wfe_linear_ce& d, const Plan& p, const void* weight, char* ws, const LceState& st) {
+  TileArgs a{};
+  a.hidden = a.weighted = st.packed;
   a.weight = p.copy_weight ? ws + p.weight : weight;
   a.weight_ld = p.copy_weight ? p.dim_pad : d.weight_stride;
   a.dim = d.dim;
   a.dim_pad = p.dim_pad;
-  a.v0 = 0;
   a.piece = a.vocab = d.vocab;
   a.row_pad = p.row_pad;
   a.head = st.head;
   a.label = st.label;
   a.zlab = st.zlab;
   a.lse = st.lse;
+  return a;
 }
 
-#define LCE_TRY(expr)                      \
-  do {                                     \
-    const hipError_t e_ = (expr);          \
-    if (e_ != hipSuccess) return e_;       \
-  } while (0)
+template <typename T, class C>
+hipError_t stats(const wfe_linear_ce& d, const TileArgs& a, int* tiles, hipStream_t stream) {
+  *tiles = tiles_of<C>(d.vocab, true);
+  const long long most = (long long)*tiles * tiles_of<C>(d.rows, false);
+  return launch<lce_logits_kernel<T, C, kStats>, C>(a, up(most, 8), stream);
+}
 
 template <typename T>
 hipError_t forward(const wfe_linear_ce& d, const void* hidden, const void* weight, const void* labels, float* loss,
                    void* state, char* ws, hipStream_t stream) {
   const Plan p = make_plan(d, weight, false, 0);
-  const LceState st = lce_state(state, d.rows);
+  const LceState st = lce_state(state, d);
   const bool none = d.reduction == WFE_REDUCE_NONE;
+  const int mean = d.reduction == WFE_REDUCE_MEAN;
   PackArgs k{};
   k.labels = labels;
   k.label_bits = d.label_bits;
@@ -747,95 +952,115 @@ hipError_t forward(const wfe_linear_ce& d, const void* hidden, const void* weigh
   k.vocab = d.vocab;
   k.per_block = (int)(d.rows <= kPackRows * 1024 ? kPackRows : up((d.rows + 1023) / 1024, 64));
   k.hidden = hidden;
-  k.packed = ws + p.packed;
+  k.packed = st.packed;
   k.st = st;
   k.losses = none ? loss : nullptr;
   const long long blocks = d.rows > 0 ? (d.rows + k.per_block - 1) / k.per_block : 1;
   lce_pack_kernel<T><<<dim3((unsigned)blocks), dim3(256), 0, stream>>>(k);
   LCE_TRY(hipGetLastError());
   if (p.copy_weight) LCE_TRY(pad_weight<T>(d, p, weight, ws, stream));
-  TileArgs a{};
-  fill_tiles(a, d, p, weight, ws, st);
+  TileArgs a = tile_args(d, p, weight, ws, st);
   a.partial = reinterpret_cast<float2*>(ws + p.partial);
-  a.a_tiles = (d.vocab + kBA - 1) / kBA;
-  a.b_tiles = (int)((d.rows + kBB - 1) / kBB);
-  if (d.rows > 0) LCE_TRY((launch_tiles<T, kStats>(a, (long long)a.a_tiles * a.b_tiles, stream)));
-  float* row_loss = reinterpret_cast<float*>(ws + p.row_loss);
+  int tiles = 0;
   if (d.rows > 0) {
-    lce_loss_kernel<<<dim3((unsigned)((d.rows + 15) / 16)), dim3(256), 0, stream>>>(
-        a.partial, a.a_tiles, p.row_pad, st, none ? loss : nullptr, row_loss);
-    LCE_TRY(hipGetLastError());
+    if (d.rows <= Small::BB) LCE_TRY((stats<T, Small>(d, a, &tiles, stream)));
+    else if (d.rows <= WFE_LROWS) LCE_TRY((stats<T, Medium>(d, a, &tiles, stream)));
+    else LCE_TRY((stats<T, Large>(d, a, &tiles, stream)));
   }
-  if (!none) lce_total_kernel<<<dim3(1), dim3(1024), 0, stream>>>(row_loss, st, loss, d.reduction == WFE_REDUCE_MEAN);
+  float* row_loss = reinterpret_cast<float*>(ws + p.row_loss);
+  float* total = none ? nullptr : loss;
+  const bool one = d.rows <= 64;
+  lce_loss_kernel<<<dim3((unsigned)(one ? 1 : (d.rows + 15) / 16)), dim3(1024), 0, stream>>>(
+      a.partial, tiles, p.row_pad, st, none ? loss : nullptr, row_loss, one ? total : nullptr, mean);
+  LCE_TRY(hipGetLastError());
+  if (total && !one) lce_total_kernel<<<dim3(1), dim3(1024), 0, stream>>>(row_loss, st, total, mean);
   return hipGetLastError();
 }
 
+template <typename T, class C>
+hipError_t gradients(const wfe_linear_ce& d, const Plan& p, GradArgs& g, char* ws, hipStream_t stream) {
+  const char* w = static_cast<const char*>(g.t.weight);
+  const int row_tiles = tiles_of<C>(d.rows, false);
+  g.rule.dim_tiles = tiles_of<C>(p.dim_pad, true);
+  g.rule.bb = C::BB;
+  g.rule.piece_steps = (p.piece + p.ke - 1) / p.ke;
+  g.rule.dwei_tiles = g.dwei ? g.rule.dim_tiles * tiles_of<C>(p.piece, false) : 0;
+  g.rule.ke = p.ke;
+  g.rule.slots = C::kSlots;
+  g.rule.most = p.splits;
+  g.t.prob_ld = p.piece;
+  for (int i = -1; i < p.pieces; ++i) {          // piece i's products beside piece i + 1's d
+    const int v0 = i < 0 ? 0 : i * p.piece, next = (i + 1) * p.piece;
+    g.next_v0 = next;
+    g.next_piece = i + 1 < p.pieces && d.rows > 0 ? (d.vocab - next < p.piece ? d.vocab - next : p.piece) : 0;
+    g.next_weight = w + (long long)next * g.t.weight_ld * p.size;
+    g.next_prob = ws + p.prob[(i + 1) & 1];
+    const long long a_tiles = tiles_of<C>(g.next_piece, true);
+    if (i < 0) {
+      if (d.rows == 0) continue;
+      TileArgs a = g.t;
+      a.v0 = 0;
+      a.piece = g.next_piece;
+      a.prob = g.next_prob;
+      LCE_TRY((launch<lce_logits_kernel<T, C, kProb>, C>(a, up(a_tiles * row_tiles, 8), stream)));
+      continue;
+    }
+    g.t.v0 = v0;
+    g.t.piece = d.vocab - v0 < p.piece ? d.vocab - v0 : p.piece;
+    g.t.weight = w + (long long)v0 * g.t.weight_ld * p.size;
+    g.t.prob = ws + p.prob[i & 1];
+    g.t.first = i == 0;
+    const long long blocks = (g.dwei ? up((long long)g.rule.dim_tiles * tiles_of<C>(g.t.piece, false), 8) : 0) +
+                             (g.dhid ? up((long long)g.rule.dim_tiles * row_tiles * p.splits, 8) : 0) +
+                             up(a_tiles * row_tiles, 8);
+    if (blocks > 0) LCE_TRY((launch<lce_grads_kernel<T, C>, C>(g, blocks, stream)));
+  }
+  return hipSuccess;
+}
+
 template <typename T>
-hipError_t backward(const wfe_linear_ce& d, const void* hidden, const void* weight, const void* state,
-                    const float* upstream, void* grad_hidden, void* grad_weight, char* ws, hipStream_t stream) {
+hipError_t backward(const wfe_linear_ce& d, const void* weight, const void* state, const float* upstream,
+                    void* grad_hidden, void* grad_weight, char* ws, hipStream_t stream) {
   const int grads = (grad_hidden ? WFE_GRAD_HIDDEN : 0) | (grad_weight ? WFE_GRAD_WEIGHT : 0);
   const Plan p = make_plan(d, weight, true, grads);
-  const LceState st = lce_state(const_cast<void*>(state), d.rows);
-  RepackArgs k{};
-  k.hidden = hidden;
-  k.inner = d.inner;
-  k.outer_stride = d.outer_stride;
-  k.inner_stride = d.inner_stride;
-  k.dim = d.dim;
-  k.dim_pad = p.dim_pad;
-  k.mean = d.reduction == WFE_REDUCE_MEAN;
-  k.per_row = d.reduction == WFE_REDUCE_NONE;
-  k.st = st;
-  k.upstream = upstream;
-  k.row_factor = reinterpret_cast<float*>(ws + p.row_factor);
-  k.factor = reinterpret_cast<float*>(ws + p.factor);
-  k.packed = ws + p.packed;
-  k.weighted = grad_weight && k.per_row ? ws + p.weighted : nullptr;
-  if (k.per_row) {
-    lce_top_kernel<<<dim3(1), dim3(1024), 0, stream>>>(upstream, st, k.factor);
-    LCE_TRY(hipGetLastError());
-  }
-  lce_repack_kernel<T><<<dim3((unsigned)(p.row_pad / kPackRows)), dim3(256), 0, stream>>>(k);
-  LCE_TRY(hipGetLastError());
+  const LceState st = lce_state(const_cast<void*>(state), d);
   if (p.copy_weight) LCE_TRY(pad_weight<T>(d, p, weight, ws, stream));
-  TileArgs a{};
-  fill_tiles(a, d, p, weight, ws, st);
-  const T* w = static_cast<const T*>(a.weight);
-  a.prob = ws + p.prob;
-  a.prob_ld = p.piece;
-  a.acc = reinterpret_cast<float*>(ws + p.acc);
-  a.splits = p.splits;
-  a.grad_weight = grad_weight;
-  a.grad_f32 = d.grad_weight_dtype == WFE_F32;
-  a.factor = k.factor;
-  const int row_tiles = (int)((d.rows + kBB - 1) / kBB);
-  const int dim_tiles = (p.dim_pad + kBA - 1) / kBA;
-  for (int v0 = 0; v0 < d.vocab; v0 += p.piece) {
-    a.v0 = v0;
-    a.piece = d.vocab - v0 < p.piece ? d.vocab - v0 : p.piece;
-    a.weight = w + (long long)v0 * a.weight_ld;
-    a.hidden = ws + p.packed;
-    a.first = v0 == 0;
-    if (d.rows > 0) {
-      a.a_tiles = (a.piece + kBA - 1) / kBA;
-      a.b_tiles = row_tiles;
-      LCE_TRY((launch_tiles<T, kProb>(a, (long long)a.a_tiles * a.b_tiles, stream)));
-      if (grad_hidden) {
-        a.a_tiles = dim_tiles;
-        LCE_TRY((launch_tiles<T, kDhid>(a, (long long)dim_tiles * row_tiles * p.splits, stream)));
-      }
-    }
-    if (grad_weight) {
-      if (k.weighted) a.hidden = k.weighted;
-      a.a_tiles = dim_tiles;
-      a.b_tiles = (a.piece + kBB - 1) / kBB;
-      LCE_TRY((launch_tiles<T, kDwei>(a, (long long)dim_tiles * a.b_tiles, stream)));
-    }
+  GradArgs g{};
+  g.t = tile_args(d, p, weight, ws, st);
+  g.t.acc = reinterpret_cast<float*>(ws + p.acc);
+  g.t.grad_weight = grad_weight;
+  g.t.grad_f32 = d.grad_weight_dtype == WFE_F32;
+  g.t.mean = d.reduction == WFE_REDUCE_MEAN;
+  g.t.factor = upstream;
+  g.dhid = grad_hidden && d.rows > 0;
+  g.dwei = grad_weight != nullptr;
+  if (g.dwei && d.reduction == WFE_REDUCE_NONE) {
+    float* top = reinterpret_cast<float*>(ws + p.top);
+    lce_top_kernel<<<dim3(1), dim3(1024), 0, stream>>>(upstream, st, top);
+    LCE_TRY(hipGetLastError());
+    lce_weigh_kernel<T><<<dim3((unsigned)(p.row_pad / 4)), dim3(256), 0, stream>>>(st.packed, ws + p.weighted, p.dim_pad,
+                                                                                st, upstream, top);
+    LCE_TRY(hipGetLastError());
+    g.t.weighted = ws + p.weighted;
+    g.t.factor = top;
   }
-  if (grad_hidden && d.rows > 0) {
-    lce_dhid_kernel<T><<<dim3((unsigned)((d.rows + 3) / 4)), dim3(256), 0, stream>>>(
-        a.acc, p.splits, p.row_pad, d.dim, p.dim_pad, d.rows, st, k.row_factor, grad_hidden,
-        d.grad_hidden_dtype == WFE_F32);
+  if (d.rows <= Small::BB) LCE_TRY((gradients<T, Small>(d, p, g, ws, stream)));
+  else if (d.rows <= WFE_LROWS) LCE_TRY((gradients<T, Medium>(d, p, g, ws, stream)));
+  else LCE_TRY((gradients<T, Large>(d, p, g, ws, stream)));
+  if (g.dhid) {
+    DhidArgs k{};
+    k.acc = g.t.acc;
+    k.rule = g.rule;
+    k.row_pad = p.row_pad;
+    k.rows = d.rows;
+    k.dim = d.dim;
+    k.dim_pad = p.dim_pad;
+    k.st = st;
+    k.upstream = upstream;
+    k.reduction = d.reduction;
+    k.out_f32 = d.grad_hidden_dtype == WFE_F32;
+    k.out = grad_hidden;
+    lce_dhid_kernel<T><<<dim3((unsigned)((d.rows + 3) / 4)), dim3(256), 0, stream>>>(k);
     LCE_TRY(hipGetLastError());
   }
   return hipSuccess;
@@ -855,15 +1080,12 @@ hipError_t launch_lce_forward(const wfe_linear_ce& d, const void* hidden, const 
   return forward<__bf16>(d, hidden, weight, labels, loss, state, ws, stream);
 }
 
-hipError_t launch_lce_backward(const wfe_linear_ce& d, const void* hidden, const void* weight, const void* state,
-                               const float* upstream, void* grad_hidden, void* grad_weight, void* workspace,
-                               hipStream_t stream) {
+hipError_t launch_lce_backward(const wfe_linear_ce& d, const void* weight, const void* state, const float* upstream,
+                               void* grad_hidden, void* grad_weight, void* workspace, hipStream_t stream) {
   char* ws = static_cast<char*>(workspace);
-  if (d.dtype == WFE_F32)
-    return backward<float>(d, hidden, weight, state, upstream, grad_hidden, grad_weight, ws, stream);
-  if (d.dtype == WFE_F16)
-    return backward<_Float16>(d, hidden, weight, state, upstream, grad_hidden, grad_weight, ws, stream);
-  return backward<__bf16>(d, hidden, weight, state, upstream, grad_hidden, grad_weight, ws, stream);
+  if (d.dtype == WFE_F32) return backward<float>(d, weight, state, upstream, grad_hidden, grad_weight, ws, stream);
+  if (d.dtype == WFE_F16) return backward<_Float16>(d, weight, state, upstream, grad_hidden, grad_weight, ws, stream);
+  return backward<__bf16>(d, weight, state, upstream, grad_hidden, grad_weight, ws, stream);
 }
 
 }  // namespace wfe

@@ -70,7 +70,7 @@ SYMBOLS = {
     "wfe_linear_ce_state_bytes": (C.c_int64, [_P]),
     "wfe_linear_ce_workspace_bytes": (C.c_int64, [_P, _P, C.c_int32, C.c_int32]),
     "wfe_linear_ce_forward": (C.c_int, [_P, _P, _P, _P, _P, _P, _P, C.c_int64, _P]),
-    "wfe_linear_ce_backward": (C.c_int, [_P, _P, _P, _P, _P, _P, _P, _P, C.c_int64, _P]),
+    "wfe_linear_ce_backward": (C.c_int, [_P, _P, _P, _P, _P, _P, _P, C.c_int64, _P]),
     "wfe_embedding": (C.c_int, [_P, _P, _P, _P, _P]),
     "wfe_embedding_workspace_bytes": (C.c_int64, [_P]),
     "wfe_embedding_backward": (C.c_int, [_P, _P, _P, _P, _P, C.c_int64, _P]),

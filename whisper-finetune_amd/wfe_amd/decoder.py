@@ -119,7 +119,7 @@ def _ce_forward(hidden, weight, labels, ignore_index, reduction):
     _lib.check(lib.wfe_linear_ce_forward(ref, hidden.data_ptr(), weight.data_ptr(), labels.data_ptr(),
                                          loss.data_ptr(), state.data_ptr(), workspace.data_ptr(), nbytes,
                                          _stream(device)))
-    return loss, state, desc, hidden, weight
+    return loss, state, desc, weight
 
 
 class _LinearCrossEntropy(torch.autograd.Function):
@@ -127,15 +127,15 @@ class _LinearCrossEntropy(torch.autograd.Function):
     def forward(ctx, hidden, weight, labels, dtype, ignore_index, reduction):
         ctx.types = (hidden.dtype, weight.dtype)
         ctx.shape = hidden.shape
-        loss, state, ctx.desc, hidden, weight = _ce_forward(hidden.to(dtype), weight.to(dtype), labels, ignore_index,
-                                                            reduction)
-        ctx.save_for_backward(hidden, weight, state)
+        loss, state, ctx.desc, weight = _ce_forward(hidden.to(dtype), weight.to(dtype), labels, ignore_index,
+                                                    reduction)
+        ctx.save_for_backward(weight, state)
         return loss
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, upstream):
-        hidden, weight, state = ctx.saved_tensors
+        weight, state = ctx.saved_tensors
         need_hidden, need_weight = ctx.needs_input_grad[:2]
         desc, device, lib = ctx.desc, weight.device, _lib.lib()
         # a gradient in float32 is written as such; any other type is the products' own, cast where the input's differs
@@ -148,7 +148,7 @@ class _LinearCrossEntropy(torch.autograd.Function):
         nbytes = lib.wfe_linear_ce_workspace_bytes(ref, weight.data_ptr(), 1, int(need_hidden) + 2 * int(need_weight))
         workspace = _workspace(nbytes, device)
         _lib.check(lib.wfe_linear_ce_backward(
-            ref, hidden.data_ptr(), weight.data_ptr(), state.data_ptr(), upstream.data_ptr(),
+            ref, weight.data_ptr(), state.data_ptr(), upstream.data_ptr(),
             grad_hidden.data_ptr() if need_hidden else None, grad_weight.data_ptr() if need_weight else None,
             workspace.data_ptr(), nbytes, _stream(device)))
         if need_hidden:
