@@ -16,6 +16,7 @@ from __future__ import annotations
 import ctypes as C
 import functools
 import types
+import weakref
 from typing import Optional
 
 import torch
@@ -46,8 +47,8 @@ def _check_matrix(name: str, weight: torch.Tensor, index_name: str, index: torch
         raise _lib.WfeError(f"{name}: tensors are on {weight.device}; an MI355X is needed, there is no CPU path")
 
 
-def _stream(device: torch.device):
-    return torch.cuda.current_stream(device).cuda_stream
+def _stream(device: torch.device) -> int:
+    return torch._C._cuda_getCurrentRawStream(device.index)
 
 
 def _workspace(nbytes: int, device: torch.device) -> torch.Tensor:
@@ -61,20 +62,30 @@ def _dense_rows(t: torch.Tensor) -> torch.Tensor:
     return t if t.shape[-1] == 1 or t.stride(-1) == 1 else t.contiguous()
 
 
-def _apply(name: str, function, *args):
-    """``function.apply(*args)``; refuses to record a call on parameters that a graph of an earlier eager call, still
-    alive, holds on to.  Autograd keeps one accumulation node per parameter while any graph refers to it, on the stream
-    it was made on; a captured backward pass would draw that stream into the capture, never to leave it, which ends the
-    process.  The node carries a note of its stream."""
-    nodes = [torch.autograd.graph.get_gradient_edge(t).node for t in args
-             if isinstance(t, torch.Tensor) and t.requires_grad and t.is_leaf]
-    if nodes:
-        stream, capturing = _stream(args[1].device), torch.cuda.is_current_stream_capturing()
-        for node in nodes:
-            if node.metadata.setdefault("wfe_stream", stream) != stream and capturing:
+class _Call:
+    """A differentiable call whose graph is alive: the graph holds this, _CALLS only knows of it."""
+    __slots__ = ("leaves", "stream", "__weakref__")
+
+    def __init__(self, leaves, stream):
+        self.leaves, self.stream = leaves, stream
+
+
+_CALLS: "weakref.WeakSet[_Call]" = weakref.WeakSet()
+
+
+def _note(name: str, *inputs: torch.Tensor) -> _Call:
+    """Refuses to record a call on parameters that the graph of an earlier eager call, still alive, holds on to.
+    Autograd keeps one accumulation node per parameter while any graph refers to it, on the stream it was made on; a
+    captured backward pass would draw that stream into the capture, never to leave it, which ends the process."""
+    leaves = [t for t in inputs if t.requires_grad and t.is_leaf]
+    call = _Call(leaves, _stream(inputs[-1].device))
+    if leaves and torch.cuda.is_current_stream_capturing():
+        for other in list(_CALLS):
+            if other.stream != call.stream and any(a is b for a in leaves for b in other.leaves):
                 raise RuntimeError(f"{name}: captured while the autograd graph of an eager call with the same parameter "
                                    "is alive; drop that call's results (or detach them) before capturing")
-    return function.apply(*args)                # (`nodes` keeps them, and their notes, until the graph does)
+    _CALLS.add(call)
+    return call
 
 
 # ---- cross entropy -----------------------------------------------------------------------------------------
@@ -108,27 +119,35 @@ def _describe(hidden, weight, labels, ignore_index, reduction):
     return desc, hidden, weight
 
 
-def _ce_forward(hidden, weight, labels, ignore_index, reduction):
+def _ce_forward(hidden, weight, labels, ignore_index, reduction, keep):
+    """(loss, what the backward pass needs if ``keep``)"""
     desc, hidden, weight = _describe(hidden, weight, labels, ignore_index, reduction)
     lib, device, ref = _lib.lib(), weight.device, C.byref(desc)
     labels = labels.contiguous()
     loss = torch.empty(labels.shape if reduction == "none" else (), dtype=torch.float32, device=device)
-    state = _workspace(lib.wfe_linear_ce_state_bytes(ref), device)
-    nbytes = lib.wfe_linear_ce_workspace_bytes(ref, weight.data_ptr(), 0, 0)
-    workspace = _workspace(nbytes, device)
-    _lib.check(lib.wfe_linear_ce_forward(ref, hidden.data_ptr(), weight.data_ptr(), labels.data_ptr(),
-                                         loss.data_ptr(), state.data_ptr(), workspace.data_ptr(), nbytes,
-                                         _stream(device)))
-    return loss, state, desc, weight
+    address = weight.data_ptr()
+    state_bytes = lib.wfe_linear_ce_state_bytes(ref)
+    nbytes = lib.wfe_linear_ce_workspace_bytes(ref, address, 0, 0)
+    if keep:
+        state, workspace = _workspace(state_bytes, device), _workspace(nbytes, device)
+        at = workspace.data_ptr()
+    else:                                       # one buffer for both
+        at = (state_bytes + 255) & -256
+        state = _workspace(at + nbytes if state_bytes >= 0 else state_bytes, device)
+        at += state.data_ptr()
+    _lib.check(lib.wfe_linear_ce_forward(ref, hidden.data_ptr(), address, labels.data_ptr(), loss.data_ptr(),
+                                         state.data_ptr(), at, nbytes, _stream(device)))
+    return loss, (state, desc, weight) if keep else None
 
 
 class _LinearCrossEntropy(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, hidden, weight, labels, dtype, ignore_index, reduction):
+    def forward(ctx, hidden, weight, labels, dtype, ignore_index, reduction, call):
+        ctx.call = call
         ctx.types = (hidden.dtype, weight.dtype)
         ctx.shape = hidden.shape
-        loss, state, ctx.desc, weight = _ce_forward(hidden.to(dtype), weight.to(dtype), labels, ignore_index,
-                                                    reduction)
+        loss, (state, ctx.desc, weight) = _ce_forward(hidden.to(dtype), weight.to(dtype), labels, ignore_index,
+                                                      reduction, True)
         ctx.save_for_backward(weight, state)
         return loss
 
@@ -155,7 +174,7 @@ class _LinearCrossEntropy(torch.autograd.Function):
             grad_hidden = grad_hidden.to(ctx.types[0])
         if need_weight:
             grad_weight = grad_weight.to(ctx.types[1])
-        return grad_hidden, grad_weight, None, None, None, None
+        return grad_hidden, grad_weight, None, None, None, None, None
 
 
 def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, labels: torch.Tensor, *,
@@ -185,8 +204,9 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, labels: tor
     elif hidden.dtype != dtype:
         raise ValueError(f"{name}: hidden is {hidden.dtype}, weight {dtype}; outside autocast they must agree")
     if torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad):
-        return _apply(name, _LinearCrossEntropy, hidden, weight, labels, dtype, int(ignore_index), reduction)
-    return _ce_forward(hidden.to(dtype), weight.to(dtype), labels, int(ignore_index), reduction)[0]
+        return _LinearCrossEntropy.apply(hidden, weight, labels, dtype, int(ignore_index), reduction,
+                                         _note(name, hidden, weight))
+    return _ce_forward(hidden.to(dtype), weight.to(dtype), labels, int(ignore_index), reduction, False)[0]
 
 
 # ---- embedding ---------------------------------------------------------------------------------------------
@@ -207,7 +227,8 @@ def _embed_forward(ids, weight, scale, padding_idx):
 
 class _TokenEmbedding(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, ids, weight, scale, padding_idx):
+    def forward(ctx, ids, weight, scale, padding_idx, call):
+        ctx.call = call
         out, ids, ctx.desc = _embed_forward(ids, weight, scale, padding_idx)
         ctx.save_for_backward(ids)
         ctx.weight_shape = weight.shape
@@ -228,7 +249,7 @@ class _TokenEmbedding(torch.autograd.Function):
         workspace = _workspace(nbytes, device)
         _lib.check(lib.wfe_embedding_backward(C.byref(desc), ids.data_ptr(), rows.data_ptr(), grad_weight.data_ptr(),
                                               workspace.data_ptr(), nbytes, _stream(device)))
-        return None, grad_weight, None, None
+        return None, grad_weight, None, None, None
 
 
 def token_embedding(ids: torch.Tensor, weight: torch.Tensor, *, scale: float = 1.0,
@@ -245,7 +266,7 @@ def token_embedding(ids: torch.Tensor, weight: torch.Tensor, *, scale: float = 1
             raise ValueError(f"{name}: padding_idx {padding_idx} outside a vocabulary of {weight.shape[0]}")
         padding_idx = int(padding_idx) % weight.shape[0]
     if torch.is_grad_enabled() and weight.requires_grad:
-        return _apply(name, _TokenEmbedding, ids, weight, float(scale), padding_idx)
+        return _TokenEmbedding.apply(ids, weight, float(scale), padding_idx, _note(name, weight))
     return _embed_forward(ids, weight, float(scale), padding_idx)[0]
 
 
