@@ -567,68 +567,66 @@ __global__ __launch_bounds__(C::kThreads, C::kWavesPerSimd) void lce_grads_kerne
 }
 
 // ---- packing ------------------------------------------------------------------------------------------------
+// (These kernels take microseconds, which first fetches of instructions dominate: the aligned case of each is a kernel
+// of its own, indices are 32 bits.)
 struct PackArgs {
   const void* labels;
-  int label_bits;
-  long long rows, inner, outer_stride, inner_stride, ignore_index;
+  int label_bits, rows, inner;
+  long long outer_stride, inner_stride, ignore_index;
   int dim, dim_pad, vocab, per_block;
   const void* hidden;
-  void* packed;
   LceState st;
   float* losses;          // per-row losses to clear for ignored rows, or null
 };
 
-__device__ inline long long label_at(const void* labels, int bits, long long n) {
+__device__ inline long long label_at(const void* labels, int bits, int n) {
   return bits == 64 ? static_cast<const long long*>(labels)[n] : static_cast<const int*>(labels)[n];
 }
 
-// one row of `dim` values to a packed row of `dim_pad`, zeros behind; factor: nullptr or the row's weight
-template <typename T>
-__device__ inline void copy_row(const T* in, T* out, int dim, int dim_pad, int lane, int lanes, float weight,
-                                bool weighted) {
+// one row of `dim` values to a packed row of `dim_pad`, zeros behind.  WIDE: dim == dim_pad and 16-byte rows
+template <typename T, bool WIDE>
+__device__ inline void copy_row(const T* in, T* out, int dim, int dim_pad, int lane) {
   constexpr int kVec = 16 / (int)sizeof(T);
-  const bool wide = (reinterpret_cast<uintptr_t>(in) & 15) == 0;
-  for (int c = lane; c < dim_pad / kVec; c += lanes) {
+  for (int d = lane * kVec; d < dim_pad; d += 64 * kVec) {
     T x[kVec];
-    const int d0 = c * kVec;
-    if (wide && d0 + kVec <= dim) __builtin_memcpy(x, __builtin_assume_aligned(in + d0, 16), 16);
+    if constexpr (WIDE) __builtin_memcpy(x, __builtin_assume_aligned(in + d, 16), 16);
     else
-      for (int e = 0; e < kVec; ++e) x[e] = d0 + e < dim ? in[d0 + e] : static_cast<T>(0.f);
-    if (weighted)
-      for (int e = 0; e < kVec; ++e) x[e] = static_cast<T>(static_cast<float>(x[e]) * weight);
-    __builtin_memcpy(__builtin_assume_aligned(out + d0, 16), x, 16);
+#pragma unroll
+      for (int e = 0; e < kVec; ++e) x[e] = d + e < dim ? in[d + e] : static_cast<T>(0.f);
+    __builtin_memcpy(__builtin_assume_aligned(out + d, 16), x, 16);
   }
 }
 
 // Block b takes rows [b per_block, ...): the kept rows before it are counted again by every block (a read of at most
 // all labels, out of L2), which saves a pass and its launch.
-constexpr int kPackRows = 16;
+constexpr int kPackRows = 4;
 
-template <typename T>
+template <typename T, bool WIDE>
 __global__ __launch_bounds__(256) void lce_pack_kernel(const PackArgs p) {
   __shared__ int counts[4];
   __shared__ int slot_of[64];
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  const long long first = (long long)blockIdx.x * p.per_block;
-  const long long last = min(first + p.per_block, p.rows);
+  const int first = blockIdx.x * p.per_block, last = min(first + p.per_block, p.rows);
   int before = 0;
-  for (long long n = threadIdx.x; n < first; n += 256) before += label_at(p.labels, p.label_bits, n) != p.ignore_index;
+#pragma unroll 4
+  for (int n = threadIdx.x; n < first; n += 256) before += label_at(p.labels, p.label_bits, n) != p.ignore_index;
   for (int d = 32; d > 0; d >>= 1) before += __shfl_xor(before, d);
   if (lane == 0) counts[wave] = before;
   __syncthreads();
   int at = counts[0] + counts[1] + counts[2] + counts[3];
-  for (long long n0 = first; n0 < last; n0 += 64) {
+#pragma unroll 1
+  for (int n0 = first; n0 < last; n0 += 64) {
     __syncthreads();
     if (wave == 0) {
-      const long long n = n0 + lane;
+      const int n = n0 + lane;
       const long long y = n < last ? label_at(p.labels, p.label_bits, n) : p.ignore_index;
-      const bool kept = n < last && y != p.ignore_index;
+      const bool kept = y != p.ignore_index;
       const unsigned long long mask = __ballot(kept);
       const int r = at + __popcll(mask & ((1ull << lane) - 1));
       slot_of[lane] = kept ? r : -1;
       if (n < last) p.st.slot[n] = kept ? r : -1;
       if (kept) {
-        p.st.index[r] = (int)n;
+        p.st.index[r] = n;
         p.st.label[r] = y >= 0 && y < p.vocab ? (int)y : -1;
         p.st.zlab[r] = __builtin_nanf("");
       } else if (n < last && p.losses) {
@@ -638,21 +636,23 @@ __global__ __launch_bounds__(256) void lce_pack_kernel(const PackArgs p) {
     }
     __syncthreads();
     at += counts[0];
-    for (int i = wave; i < min(64ll, last - n0); i += 4) {
+#pragma unroll 1
+    for (int i = wave; i < min(64, last - n0); i += 4) {
       const int r = slot_of[i];
       if (r < 0) continue;
-      const long long n = n0 + i;
-      const T* in = static_cast<const T*>(p.hidden) + (n / p.inner) * p.outer_stride + (n % p.inner) * p.inner_stride;
-      copy_row<T>(in, static_cast<T*>(p.packed) + (long long)r * p.dim_pad, p.dim, p.dim_pad, lane, 64, 1.f, false);
+      const unsigned n = n0 + i, outer = n / (unsigned)p.inner;
+      const T* in = static_cast<const T*>(p.hidden) + outer * p.outer_stride + (n - outer * p.inner) * p.inner_stride;
+      copy_row<T, WIDE>(in, static_cast<T*>(p.st.packed) + (long long)r * p.dim_pad, p.dim, p.dim_pad, lane);
     }
   }
   if (blockIdx.x == gridDim.x - 1) {         // knows the number of kept rows
     if (threadIdx.x == 0) p.st.head[0] = at;
     // DWEI goes over the rows in whole K tiles: zeros up to there (rows further on reach only sums that nobody reads)
-    const long long end = ((long long)at + kPadRows - 1) / kPadRows * kPadRows;
-    const long long vecs = (end - at) * p.dim_pad * (long long)sizeof(T) / 16;
-    f32x4* out = reinterpret_cast<f32x4*>(static_cast<T*>(p.packed) + (long long)at * p.dim_pad);
-    for (long long i = threadIdx.x; i < vecs; i += 256) out[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const int end = (at + kPadRows - 1) / kPadRows * kPadRows;
+    const int vecs = (end - at) * (p.dim_pad / (16 / (int)sizeof(T)));
+    f32x4* out = reinterpret_cast<f32x4*>(static_cast<T*>(p.st.packed) + (long long)at * p.dim_pad);
+#pragma unroll 1
+    for (int i = threadIdx.x; i < vecs; i += 256) out[i] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
 }
 
@@ -676,13 +676,20 @@ __global__ __launch_bounds__(1024) void lce_top_kernel(const float* upstream, Lc
 template <typename T>
 __global__ __launch_bounds__(256) void lce_weigh_kernel(const void* packed, void* weighted, int dim_pad, LceState st,
                                                         const float* upstream, const float* top) {
+  constexpr int kVec = 16 / (int)sizeof(T);
   const int count = st.head[0];
-  const long long r = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int r = blockIdx.x * 4 + (threadIdx.x >> 6);
   if (r >= (count + kPadRows - 1) / kPadRows * kPadRows) return;
   const bool kept = r < count;
-  const float g = kept ? upstream[st.index[r]] : 0.f;
-  copy_row<T>(static_cast<const T*>(packed) + r * dim_pad, static_cast<T*>(weighted) + r * dim_pad,
-              kept ? dim_pad : 0, dim_pad, threadIdx.x & 63, 64, *top > 0.f ? g / *top : g, true);
+  float g = kept ? upstream[st.index[r]] : 0.f;
+  if (*top > 0.f) g /= *top;
+  for (int d = (threadIdx.x & 63) * kVec; d < dim_pad; d += 64 * kVec) {
+    T x[kVec];
+    __builtin_memcpy(x, __builtin_assume_aligned(static_cast<const T*>(packed) + (long long)r * dim_pad + d, 16), 16);
+#pragma unroll
+    for (int e = 0; e < kVec; ++e) x[e] = kept ? static_cast<T>(static_cast<float>(x[e]) * g) : static_cast<T>(0.f);
+    __builtin_memcpy(__builtin_assume_aligned(static_cast<T*>(weighted) + (long long)r * dim_pad + d, 16), x, 16);
+  }
 }
 
 // W with rows that the tiles cannot read in place (odd sizes, strides or alignment): one padded copy
@@ -691,7 +698,7 @@ __global__ __launch_bounds__(256) void lce_pad_weight_kernel(const T* weight, lo
                                                              int dim_pad, int vocab) {
   const int v = blockIdx.x * 4 + (threadIdx.x >> 6);
   if (v < vocab)
-    copy_row<T>(weight + (long long)v * ld, out + (long long)v * dim_pad, dim, dim_pad, threadIdx.x & 63, 64, 1.f, false);
+    copy_row<T, false>(weight + (long long)v * ld, out + (long long)v * dim_pad, dim, dim_pad, threadIdx.x & 63);
 }
 
 // ---- losses out of the tiles' statistics --------------------------------------------------------------------
@@ -762,12 +769,12 @@ __global__ __launch_bounds__(1024) void lce_total_kernel(const float* row_loss, 
   sum_losses(row_loss, st.head[0], total, mean);
 }
 
-// dh: the splits' sums, times g, to every row's place; zeros for ignored rows.  One wave per row.
+// dh: the splits' sums, times g, to every row's place; zeros for ignored rows.  A wave takes 256 columns of a row.
 struct DhidArgs {
   const float* acc;
   SplitRule rule;
-  long long row_pad, rows;
-  int dim, dim_pad;
+  long long row_pad;
+  int rows, dim, dim_pad;
   LceState st;
   const float* upstream;
   int reduction, out_f32;
@@ -776,38 +783,36 @@ struct DhidArgs {
 
 template <typename T>
 __global__ __launch_bounds__(256) void lce_dhid_kernel(const DhidArgs p) {
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  const long long n = (long long)blockIdx.x * 4 + wave;
-  if (n >= p.rows) return;
+  const int n = blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int d = (blockIdx.y * 64 + (threadIdx.x & 63)) * 4;
+  if (n >= p.rows || d >= p.dim) return;
   const int r = p.st.slot[n], count = p.st.head[0];
-  const bool kept = r >= 0;
-  const int splits = kept ? dhid_splits(p.rule, count) : 0;
-  float g = 0.f;
-  if (kept) {
-    g = p.upstream[p.reduction == WFE_REDUCE_NONE ? n : 0];
+  f32x4 s = {0.f, 0.f, 0.f, 0.f};
+  if (r >= 0) {
+    const int splits = dhid_splits(p.rule, count);
+    float g = p.upstream[p.reduction == WFE_REDUCE_NONE ? n : 0] * (1.f / Elem<T>::kScale);
     if (p.reduction == WFE_REDUCE_MEAN) g /= (float)count;
-    g *= 1.f / Elem<T>::kScale;
-  }
-  const bool whole = (p.dim & 3) == 0;
-  for (int d = lane * 4; d < p.dim; d += 256) {
-    f32x4 s = {0.f, 0.f, 0.f, 0.f};
     const float* from = p.acc + (long long)r * p.dim_pad + d;
-    for (int i = 0; i < splits; ++i) s += *reinterpret_cast<const f32x4*>(from + (long long)i * p.row_pad * p.dim_pad);
-    if (kept) s *= g;
-    const long long at = n * p.dim + d;
-    if (p.out_f32) {
-      float* out = static_cast<float*>(p.out) + at;
-      if (whole) *reinterpret_cast<f32x4*>(out) = s;
-      else
-        for (int e = 0; e < 4 && d + e < p.dim; ++e) out[e] = s[e];
-    } else {
-      T* out = static_cast<T*>(p.out) + at;
-      T x[4];
-      for (int e = 0; e < 4; ++e) x[e] = static_cast<T>(s[e]);
-      if (whole) __builtin_memcpy(__builtin_assume_aligned(out, 4 * sizeof(T)), x, sizeof x);
-      else
-        for (int e = 0; e < 4 && d + e < p.dim; ++e) out[e] = x[e];
-    }
+    const long long step = p.row_pad * p.dim_pad;
+#pragma unroll 8
+    for (int i = 0; i < splits; ++i) s += *reinterpret_cast<const f32x4*>(from + i * step);
+    s *= g;
+  }
+  const long long at = (long long)n * p.dim + d;
+  const bool whole = (p.dim & 3) == 0;
+  if (p.out_f32) {
+    float* out = static_cast<float*>(p.out) + at;
+    if (whole) *reinterpret_cast<f32x4*>(out) = s;
+    else
+      for (int e = 0; e < 4 && d + e < p.dim; ++e) out[e] = s[e];
+  } else {
+    T* out = static_cast<T*>(p.out) + at;
+    T x[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] = static_cast<T>(s[e]);
+    if (whole) __builtin_memcpy(__builtin_assume_aligned(out, 4 * sizeof(T)), x, sizeof x);
+    else
+      for (int e = 0; e < 4 && d + e < p.dim; ++e) out[e] = x[e];
   }
 }
 
@@ -942,21 +947,24 @@ hipError_t forward(const wfe_linear_ce& d, const void* hidden, const void* weigh
   PackArgs k{};
   k.labels = labels;
   k.label_bits = d.label_bits;
-  k.rows = d.rows;
-  k.inner = d.inner;
+  k.rows = (int)d.rows;
+  k.inner = (int)(d.inner < d.rows ? d.inner : d.rows > 0 ? d.rows : 1);
   k.outer_stride = d.outer_stride;
   k.inner_stride = d.inner_stride;
   k.ignore_index = d.ignore_index;
   k.dim = d.dim;
   k.dim_pad = p.dim_pad;
   k.vocab = d.vocab;
-  k.per_block = (int)(d.rows <= kPackRows * 1024 ? kPackRows : up((d.rows + 1023) / 1024, 64));
+  k.per_block = (int)up(d.rows > 0 ? (d.rows + 1023) / 1024 : 1, kPackRows);      // at most 1024 blocks
   k.hidden = hidden;
-  k.packed = st.packed;
   k.st = st;
   k.losses = none ? loss : nullptr;
   const long long blocks = d.rows > 0 ? (d.rows + k.per_block - 1) / k.per_block : 1;
-  lce_pack_kernel<T><<<dim3((unsigned)blocks), dim3(256), 0, stream>>>(k);
+  constexpr int kVec = 16 / (int)sizeof(T);
+  const bool wide = d.dim == p.dim_pad && reinterpret_cast<uintptr_t>(hidden) % 16 == 0 && d.outer_stride % kVec == 0 &&
+                    d.inner_stride % kVec == 0;
+  if (wide) lce_pack_kernel<T, true><<<dim3((unsigned)blocks), dim3(256), 0, stream>>>(k);
+  else lce_pack_kernel<T, false><<<dim3((unsigned)blocks), dim3(256), 0, stream>>>(k);
   LCE_TRY(hipGetLastError());
   if (p.copy_weight) LCE_TRY(pad_weight<T>(d, p, weight, ws, stream));
   TileArgs a = tile_args(d, p, weight, ws, st);
@@ -1052,7 +1060,7 @@ hipError_t backward(const wfe_linear_ce& d, const void* weight, const void* stat
     k.acc = g.t.acc;
     k.rule = g.rule;
     k.row_pad = p.row_pad;
-    k.rows = d.rows;
+    k.rows = (int)d.rows;
     k.dim = d.dim;
     k.dim_pad = p.dim_pad;
     k.st = st;
@@ -1060,7 +1068,7 @@ hipError_t backward(const wfe_linear_ce& d, const void* weight, const void* stat
     k.reduction = d.reduction;
     k.out_f32 = d.grad_hidden_dtype == WFE_F32;
     k.out = grad_hidden;
-    lce_dhid_kernel<T><<<dim3((unsigned)((d.rows + 3) / 4)), dim3(256), 0, stream>>>(k);
+    lce_dhid_kernel<T><<<dim3((unsigned)((d.rows + 3) / 4), (d.dim + 255) / 256), dim3(256), 0, stream>>>(k);
     LCE_TRY(hipGetLastError());
   }
   return hipSuccess;
