@@ -73,12 +73,13 @@ __device__ inline float exp_of(float x) { return __builtin_amdgcn_exp2f(x * kLog
 // An operand tile in LDS is either rows x 64 bytes of K ("along": K contiguous in memory) or K rows x columns
 // ("across": K strided in memory, transposed by the read).  16-byte chunks of a row are permuted by an exclusive or
 // so that the lanes of a fragment read meet different banks:
-//   along           rows of 4 chunks, 4 rows cover the banks: the rows 4 apart take different chunks
+//   along           rows of 4 chunks, 4 rows cover the banks: rows 4 apart take different pairs of chunks (a 16-byte
+//                   read serves 8 lanes of one chunk number with 8 of the next at a time)
 //   across, 2 byte  pairs of chunks (a transposing read takes 32 bytes of each of 4 rows); 8 rows 0..3, 8..11 apart
 //   across, 4 byte  groups of four chunks; 4 rows 4 apart
 template <typename T, bool ACROSS, int N>
 __device__ inline int swizzle(int row) {
-  if constexpr (!ACROSS) return (row >> 2) & 3;
+  if constexpr (!ACROSS) return (row >> 1) & 2;
   else if constexpr (sizeof(T) == 2) return (((row & 3) | ((row >> 1) & 4)) & (N / 16 - 1)) << 1;
   else return (((row >> 2) & 3) & (N / 16 - 1)) << 2;
 }
@@ -817,16 +818,25 @@ __global__ __launch_bounds__(256) void lce_dhid_kernel(const DhidArgs p) {
 }
 
 // ---- host side ----------------------------------------------------------------------------------------------
-#ifndef WFE_L
-#define WFE_L 256, 256, 4, 2, 4, 1
-#define WFE_M 256, 128, 2, 2, 3, 2
-#define WFE_S 128, 32, 4, 1, 4, 4
-#define WFE_LROWS 768
+using Large = Cfg<256, 256, 4, 2, 4, 1>;
+using Medium = Cfg<256, 128, 2, 2, 3, 2>;
+using Fine = Cfg<128, 64, 2, 2, 4, 3>;         // float32, whose products take eight times as long per byte
+using Small = Cfg<128, 32, 4, 1, 4, 4>;
+constexpr int kStatsRows = 128;                // fewest vocabulary rows of a tile: room for the statistics
+constexpr int kLargeRows = 768;
+#ifndef WFE_PB
+#define WFE_PB 128
 #endif
-using Large = Cfg<WFE_L>;
-using Medium = Cfg<WFE_M>;
-using Small = Cfg<WFE_S>;
-constexpr long long kPieceBytes = 128ll << 20;     // most that the d of one piece takes; two pieces are held
+constexpr long long kPieceBytes = (long long)WFE_PB << 20;     // most that the d of one piece takes; two pieces are held
+
+// calls f with the tile that suits this many rows
+template <typename T, class F>
+hipError_t with_tile(int64_t rows, F f) {
+  if (rows <= Small::BB) return f(Small{});
+  if (rows > kLargeRows) return f(Large{});
+  if constexpr (sizeof(T) == 4) return f(Fine{});
+  else return f(Medium{});
+}
 
 long long up(long long x, long long to) { return (x + to - 1) / to * to; }
 
@@ -859,7 +869,7 @@ Plan make_plan(const wfe_linear_ce& d, const void* weight, bool backward, int gr
   };
   if (p.copy_weight) p.weight = take((long long)d.vocab * p.dim_pad * p.size);
   if (!backward) {
-    p.partial = take(up(d.vocab, Small::BA) / Small::BA * p.row_pad * 8);
+    p.partial = take(up(d.vocab, kStatsRows) / kStatsRows * p.row_pad * 8);
     p.row_loss = take(p.row_pad * 4);
   } else {
     const long long all = up(d.vocab, kLceRowPad);
@@ -932,6 +942,7 @@ TileArgs tile_args(const wfe_linear_ce& d, const Plan& p, const void* weight, ch
 
 template <typename T, class C>
 hipError_t stats(const wfe_linear_ce& d, const TileArgs& a, int* tiles, hipStream_t stream) {
+  static_assert(C::BA >= kStatsRows, "room for the statistics");
   *tiles = tiles_of<C>(d.vocab, true);
   const long long most = (long long)*tiles * tiles_of<C>(d.rows, false);
   return launch<lce_logits_kernel<T, C, kStats>, C>(a, up(most, 8), stream);
@@ -971,9 +982,7 @@ hipError_t forward(const wfe_linear_ce& d, const void* hidden, const void* weigh
   a.partial = reinterpret_cast<float2*>(ws + p.partial);
   int tiles = 0;
   if (d.rows > 0) {
-    if (d.rows <= Small::BB) LCE_TRY((stats<T, Small>(d, a, &tiles, stream)));
-    else if (d.rows <= WFE_LROWS) LCE_TRY((stats<T, Medium>(d, a, &tiles, stream)));
-    else LCE_TRY((stats<T, Large>(d, a, &tiles, stream)));
+    LCE_TRY(with_tile<T>(d.rows, [&](auto c) { return stats<T, decltype(c)>(d, a, &tiles, stream); }));
   }
   float* row_loss = reinterpret_cast<float*>(ws + p.row_loss);
   float* total = none ? nullptr : loss;
@@ -1052,9 +1061,7 @@ hipError_t backward(const wfe_linear_ce& d, const void* weight, const void* stat
     g.t.weighted = ws + p.weighted;
     g.t.factor = top;
   }
-  if (d.rows <= Small::BB) LCE_TRY((gradients<T, Small>(d, p, g, ws, stream)));
-  else if (d.rows <= WFE_LROWS) LCE_TRY((gradients<T, Medium>(d, p, g, ws, stream)));
-  else LCE_TRY((gradients<T, Large>(d, p, g, ws, stream)));
+  LCE_TRY(with_tile<T>(d.rows, [&](auto c) { return gradients<T, decltype(c)>(d, p, g, ws, stream); }));
   if (g.dhid) {
     DhidArgs k{};
     k.acc = g.t.acc;
