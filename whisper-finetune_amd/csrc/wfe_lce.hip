@@ -218,10 +218,10 @@ struct TileArgs {
   int mean;
 };
 
-// The id-th of `a_tiles` x `b_tiles` tiles of part `split` of `splits` of K.  smem: C::kLds bytes.
+// The id-th of `a_tiles` x `b_tiles` tiles, from column b_first on, of part `split` of `splits` of K.  smem: C::kLds bytes.
 template <typename T, class C, int MODE>
-__device__ __forceinline__ void run_tile(const TileArgs& p, int count, int id, int a_tiles, int b_tiles, int splits,
-                                         char* smem) {
+__device__ __forceinline__ void run_tile(const TileArgs& p, int count, int id, int a_tiles, int b_tiles, int b_first,
+                                         int splits, char* smem) {
   constexpr bool kAAcross = MODE == kDhid || MODE == kDwei;
   constexpr bool kBAcross = MODE == kDwei;
   constexpr int BA = C::BA, BB = C::BB, WA = C::WA, WB = C::WB, kStages = C::S, kStage = C::kStage;
@@ -237,7 +237,7 @@ __device__ __forceinline__ void run_tile(const TileArgs& p, int count, int id, i
   const int rest = id - group * kGroup * a_tiles;
   const int in_group = min(kGroup, b_tiles - group * kGroup);
   const int ta = rest / in_group, tb = group * kGroup + rest % in_group;
-  const int a0 = ta * BA, b0 = tb * BB;
+  const int a0 = ta * BA, b0 = b_first + tb * BB;
 
   // K range, in tiles
   int k_first = 0, k_tiles;
@@ -481,15 +481,53 @@ __device__ inline int tile_of(int b, int tiles) {
   return id < tiles ? id : -1;
 }
 
+// The kept rows as strips of a tile's width; the rows that are left over, if they are few, take a narrower tile of the
+// same threads (552 rows as 2 x 256 + 64 instead of 3 x 256).
+template <class C>
+struct Strips {
+  static constexpr bool kNarrow = C::BB == 256;
+  using Half = Cfg<C::BA, kNarrow ? 128 : C::BB, C::WA, C::WB, C::S, C::PER>;
+  using Quarter = Cfg<C::BA, kNarrow ? 64 : C::BB, C::WA, C::WB, C::S, C::PER>;
+  int whole, rest;              // strips of C::BB rows; rows of the narrow strip: 0, 64 or 128
+  __device__ explicit Strips(int count) {
+    const int over = count % C::BB;
+    rest = !kNarrow || over == 0 || over > 128 ? 0 : over > 64 ? 128 : 64;
+    whole = count / C::BB + (over > 0 && rest == 0);
+  }
+};
+
+// Block b of the tiles over all strips, whole ones first; false: behind the last block
+template <typename T, class C, int MODE>
+__device__ __forceinline__ bool run_strips(const TileArgs& p, int count, int& b, int a_tiles, int splits, char* smem) {
+  using S = Strips<C>;
+  const S s(count);
+  const int tiles = a_tiles * s.whole * splits;
+  if (b < run_blocks(tiles)) {
+    const int id = tile_of(b, tiles);
+    if (id >= 0) run_tile<T, C, MODE>(p, count, id, a_tiles, s.whole, 0, splits, smem);
+    return true;
+  }
+  b -= run_blocks(tiles);
+  if constexpr (S::kNarrow) {
+    const int narrow = s.rest > 0 ? a_tiles * splits : 0;
+    if (b < run_blocks(narrow)) {
+      const int id = tile_of(b, narrow);
+      if (id >= 0) {
+        if (s.rest == 64) run_tile<T, typename S::Quarter, MODE>(p, count, id, a_tiles, 1, s.whole * C::BB, splits, smem);
+        else run_tile<T, typename S::Half, MODE>(p, count, id, a_tiles, 1, s.whole * C::BB, splits, smem);
+      }
+      return true;
+    }
+    b -= run_blocks(narrow);
+  }
+  return false;
+}
+
 template <typename T, class C, int MODE>
 __global__ __launch_bounds__(C::kThreads, C::kWavesPerSimd) void lce_logits_kernel(const TileArgs p) {
   extern __shared__ __align__(1024) char smem[];
-  const int count = p.head[0];
-  const int a_tiles = (p.piece + C::BA - 1) / C::BA, b_tiles = (count + C::BB - 1) / C::BB;
-  const int tiles = a_tiles * b_tiles;
-  if ((int)blockIdx.x >= run_blocks(tiles)) return;
-  const int id = tile_of(blockIdx.x, tiles);
-  if (id >= 0) run_tile<T, C, MODE>(p, count, id, a_tiles, b_tiles, 1, smem);
+  int b = blockIdx.x;
+  run_strips<T, C, MODE>(p, p.head[0], b, (p.piece + C::BA - 1) / C::BA, 1, smem);
 }
 
 // DHID has few tiles of its own, so its K, the vocabulary, is split.  Beside DWEI: parts of half a CU's share of all
@@ -534,36 +572,25 @@ template <typename T, class C>
 __global__ __launch_bounds__(C::kThreads, C::kWavesPerSimd) void lce_grads_kernel(const GradArgs g) {
   extern __shared__ __align__(1024) char smem[];
   const int count = g.t.head[0];
-  const int row_tiles = (count + C::BB - 1) / C::BB;
   const int dim_tiles = g.rule.dim_tiles;
   int b = blockIdx.x;
   if (g.dwei) {
     const int b_tiles = (g.t.piece + C::BB - 1) / C::BB, tiles = dim_tiles * b_tiles;
     if (b < run_blocks(tiles)) {
       const int id = tile_of(b, tiles);
-      if (id >= 0) run_tile<T, C, kDwei>(g.t, count, id, dim_tiles, b_tiles, 1, smem);
+      if (id >= 0) run_tile<T, C, kDwei>(g.t, count, id, dim_tiles, b_tiles, 0, 1, smem);
       return;
     }
     b -= run_blocks(tiles);
   }
-  if (g.dhid) {
-    const int splits = dhid_splits(g.rule, count), tiles = dim_tiles * row_tiles * splits;
-    if (b < run_blocks(tiles)) {
-      const int id = tile_of(b, tiles);
-      if (id >= 0) run_tile<T, C, kDhid>(g.t, count, id, dim_tiles, row_tiles, splits, smem);
-      return;
-    }
-    b -= run_blocks(tiles);
-  }
+  if (g.dhid && run_strips<T, C, kDhid>(g.t, count, b, dim_tiles, dhid_splits(g.rule, count), smem)) return;
   if (g.next_piece > 0) {
     TileArgs p = g.t;
     p.v0 = g.next_v0;
     p.piece = g.next_piece;
     p.weight = g.next_weight;
     p.prob = g.next_prob;
-    const int a_tiles = (p.piece + C::BA - 1) / C::BA, tiles = a_tiles * row_tiles;
-    const int id = b < run_blocks(tiles) ? tile_of(b, tiles) : -1;
-    if (id >= 0) run_tile<T, C, kProb>(p, count, id, a_tiles, row_tiles, 1, smem);
+    run_strips<T, C, kProb>(p, count, b, (p.piece + C::BA - 1) / C::BA, 1, smem);
   }
 }
 
@@ -823,7 +850,10 @@ using Medium = Cfg<256, 128, 2, 2, 3, 2>;
 using Fine = Cfg<128, 64, 2, 2, 4, 3>;         // float32, whose products take eight times as long per byte
 using Small = Cfg<128, 32, 4, 1, 4, 4>;
 constexpr int kStatsRows = 128;                // fewest vocabulary rows of a tile: room for the statistics
-constexpr int kLargeRows = 768;
+#ifndef WFE_LR
+#define WFE_LR 192
+#endif
+constexpr int kLargeRows = WFE_LR;
 #ifndef WFE_PB
 #define WFE_PB 128
 #endif
@@ -940,12 +970,17 @@ TileArgs tile_args(const wfe_linear_ce& d, const Plan& p, const void* weight, ch
   return a;
 }
 
+// The most blocks that the strips of up to `rows` rows take with `tiles` tiles each
+template <class C>
+long long strip_blocks(long long tiles, int64_t rows) {
+  return up(tiles * tiles_of<C>(rows, false), 8) + (Strips<C>::kNarrow ? up(tiles, 8) : 0);
+}
+
 template <typename T, class C>
 hipError_t stats(const wfe_linear_ce& d, const TileArgs& a, int* tiles, hipStream_t stream) {
   static_assert(C::BA >= kStatsRows, "room for the statistics");
   *tiles = tiles_of<C>(d.vocab, true);
-  const long long most = (long long)*tiles * tiles_of<C>(d.rows, false);
-  return launch<lce_logits_kernel<T, C, kStats>, C>(a, up(most, 8), stream);
+  return launch<lce_logits_kernel<T, C, kStats>, C>(a, strip_blocks<C>(*tiles, d.rows), stream);
 }
 
 template <typename T>
@@ -997,7 +1032,6 @@ hipError_t forward(const wfe_linear_ce& d, const void* hidden, const void* weigh
 template <typename T, class C>
 hipError_t gradients(const wfe_linear_ce& d, const Plan& p, GradArgs& g, char* ws, hipStream_t stream) {
   const char* w = static_cast<const char*>(g.t.weight);
-  const int row_tiles = tiles_of<C>(d.rows, false);
   g.rule.dim_tiles = tiles_of<C>(p.dim_pad, true);
   g.rule.bb = C::BB;
   g.rule.piece_steps = (p.piece + p.ke - 1) / p.ke;
@@ -1019,7 +1053,7 @@ hipError_t gradients(const wfe_linear_ce& d, const Plan& p, GradArgs& g, char* w
       a.v0 = 0;
       a.piece = g.next_piece;
       a.prob = g.next_prob;
-      LCE_TRY((launch<lce_logits_kernel<T, C, kProb>, C>(a, up(a_tiles * row_tiles, 8), stream)));
+      LCE_TRY((launch<lce_logits_kernel<T, C, kProb>, C>(a, strip_blocks<C>(a_tiles, d.rows), stream)));
       continue;
     }
     g.t.v0 = v0;
@@ -1028,8 +1062,8 @@ hipError_t gradients(const wfe_linear_ce& d, const Plan& p, GradArgs& g, char* w
     g.t.prob = ws + p.prob[i & 1];
     g.t.first = i == 0;
     const long long blocks = (g.dwei ? up((long long)g.rule.dim_tiles * tiles_of<C>(g.t.piece, false), 8) : 0) +
-                             (g.dhid ? up((long long)g.rule.dim_tiles * row_tiles * p.splits, 8) : 0) +
-                             up(a_tiles * row_tiles, 8);
+                             (g.dhid ? strip_blocks<C>((long long)g.rule.dim_tiles * p.splits, d.rows) : 0) +
+                             (g.next_piece > 0 ? strip_blocks<C>(a_tiles, d.rows) : 0);
     if (blocks > 0) LCE_TRY((launch<lce_grads_kernel<T, C>, C>(g, blocks, stream)));
   }
   return hipSuccess;
