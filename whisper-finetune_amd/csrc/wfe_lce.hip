@@ -6,7 +6,7 @@
 //
 // Rows whose label is ignore_index are dropped first: lce_pack_kernel copies the kept ones together, every product
 // after it runs over the kept rows only, whose number stays on the device.  All four products are one tile routine that
-// multiplies 16-byte K fragments out of LDS:
+// multiplies K fragments out of LDS:
 //   STATS  z tiles, reduced in registers to a maximum and a sum of exponentials per row and vocabulary tile
 //   PROB   z tiles again, written as d for a piece of the vocabulary
 //   DHID   dh += d W over that piece, in float32
@@ -26,60 +26,82 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x8 __attribute__((ext_vector_type(8)));
 
-// 16 bytes of K of one row (or column) per lane: 8 values of 2 bytes or 4 of 4
-union Frag {
-  i32x4 i;
-  bf16x8 b;
-  f16x8 h;
-  f32x4 f;
-  s16x4 s[2];
-};
-
+// Element types.  Frag: 32 K of 16 rows (or columns), a lane's share; lane group g = lane / 16 holds k = 8 g .. 8 g + 7
+// of 2-byte types, and k = 4 g .. 4 g + 3 and 16 + 4 g .. 16 + 4 g + 3 of float: any order does that is the same on both
+// sides of a product.
 template <typename T> struct Elem;
 template <> struct Elem<__bf16> {
+  union Frag { i32x4 i; bf16x8 b; s16x4 s[2]; };
   static __device__ f32x4 mma(const Frag& a, const Frag& b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.b, b.b, c, 0, 0, 0);
   }
   static constexpr float kScale = 1.0f;
 };
 template <> struct Elem<_Float16> {
+  union Frag { i32x4 i; f16x8 h; s16x4 s[2]; };
   static __device__ f32x4 mma(const Frag& a, const Frag& b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a.h, b.h, c, 0, 0, 0);
   }
   // d is in [-1, 1]: stored times 2^14 so that small probabilities stay clear of the subnormals
   static constexpr float kScale = 16384.0f;
 };
+// float32 products on the bfloat16 matrix instructions, which do 16 times the work of the float32 ones per cycle: a
+// value is the exact sum of three bfloat16 (8 + 8 + 8 of its 24 bits, each the rounding of what is left), and of the nine
+// partial products the six down to 2^-16 of the whole are added up, smallest first.  What is left out is under 2^-26 of a
+// product, a quarter of what rounding it to float32 costs.  Infinities (inf - inf while splitting) come out as NaN:
+// run_tile repeats such a tile with the float32 instructions.
 template <> struct Elem<float> {
-  // lane group g holds k = 4 g .. 4 g + 3 of a 16-deep step; the i-th instruction takes every group's i-th value,
-  // the same on both sides
-  static __device__ f32x4 mma(const Frag& a, const Frag& b, f32x4 c) {
+  struct Frag { f32x4 x[2]; };
+  struct Parts { bf16x8 hi, mid, lo; };
+  static __device__ Parts split(const Frag& f) {
+    const f32x8 x = __builtin_shufflevector(f.x[0], f.x[1], 0, 1, 2, 3, 4, 5, 6, 7);
+    Parts p;
+    p.hi = __builtin_convertvector(x, bf16x8);
+    const f32x8 r = x - __builtin_convertvector(p.hi, f32x8);
+    p.mid = __builtin_convertvector(r, bf16x8);
+    p.lo = __builtin_convertvector(r - __builtin_convertvector(p.mid, f32x8), bf16x8);
+    return p;
+  }
+  static __device__ f32x4 mma(const Parts& a, const Parts& b, f32x4 c) {
+    c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.lo, b.hi, c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.hi, b.lo, c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.mid, b.mid, c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.mid, b.hi, c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.hi, b.mid, c, 0, 0, 0);
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.hi, b.hi, c, 0, 0, 0);
+  }
+  static __device__ f32x4 mma_exact(const Frag& a, const Frag& b, f32x4 c) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a.f[i], b.f[i], c, 0, 0, 0);
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a.x[h][i], b.x[h][i], c, 0, 0, 0);
     return c;
   }
   static constexpr float kScale = 1.0f;
 };
 
-constexpr int kKBytes = 64;                                // depth of a K tile in bytes: one MFMA step of 2-byte types
+constexpr int kKElems = 32;                                // depth of a K tile
+template <typename T> constexpr int kKBytes = kKElems * (int)sizeof(T);
 constexpr int kPadBytes = 128;                             // packed rows are whole multiples of this
 constexpr int kPadRows = 64;                               // zeros follow the kept rows up to a multiple of this
-template <typename T> constexpr int kKElems = kKBytes / (int)sizeof(T);
 constexpr float kLog2e = 1.44269504088896340736f;
 
 __device__ inline float exp_of(float x) { return __builtin_amdgcn_exp2f(x * kLog2e); }
 
 // ---- operands -------------------------------------------------------------------------------------------
-// An operand tile in LDS is either rows x 64 bytes of K ("along": K contiguous in memory) or K rows x columns
+// An operand tile in LDS is either rows x 32 of K ("along": K contiguous in memory) or K rows x columns
 // ("across": K strided in memory, transposed by the read).  16-byte chunks of a row are permuted by an exclusive or
 // so that the lanes of a fragment read meet different banks:
-//   along           rows of 4 chunks, 4 rows cover the banks: rows 4 apart take different pairs of chunks (a 16-byte
+//   along, 2 byte   rows of 4 chunks, 4 rows cover the banks: rows 4 apart take different pairs of chunks (a 16-byte
 //                   read serves 8 lanes of one chunk number with 8 of the next at a time)
+//   along, 4 byte   rows of 8 chunks: chunk ^ (row & 7)
 //   across, 2 byte  pairs of chunks (a transposing read takes 32 bytes of each of 4 rows); 8 rows 0..3, 8..11 apart
 //   across, 4 byte  groups of four chunks; 4 rows 4 apart
 template <typename T, bool ACROSS, int N>
 __device__ inline int swizzle(int row) {
-  if constexpr (!ACROSS) return (row >> 1) & 2;
+  if constexpr (!ACROSS) return sizeof(T) == 2 ? (row >> 1) & 2 : row & 7;
   else if constexpr (sizeof(T) == 2) return (((row & 3) | ((row >> 1) & 4)) & (N / 16 - 1)) << 1;
   else return (((row >> 2) & 3) & (N / 16 - 1)) << 2;
 }
@@ -87,9 +109,9 @@ __device__ inline int swizzle(int row) {
 // Loads tiles of N rows (or columns) with NW waves, 1024 bytes per wave and instruction straight into LDS.
 template <typename T, bool ACROSS, int N, int NW>
 struct Loader {
-  static constexpr int kRowBytes = ACROSS ? N * (int)sizeof(T) : kKBytes;
+  static constexpr int kRowBytes = ACROSS ? N * (int)sizeof(T) : kKBytes<T>;
   static constexpr int kChunks = kRowBytes / 16;
-  static constexpr int kTileBytes = N * kKBytes;
+  static constexpr int kTileBytes = N * kKBytes<T>;
   static constexpr int kInstrs = kTileBytes / 1024;
   static constexpr int kPer = (kInstrs + NW - 1) / NW;
   const char* base;
@@ -108,11 +130,11 @@ struct Loader {
     ld = ld_elems * (long long)sizeof(T);
     if constexpr (ACROSS) {
       base = reinterpret_cast<const char*>(p) + k0 * ld + (long long)first * sizeof(T);
-      step = ld * kKElems<T>;
+      step = ld * kKElems;
       k_left = (int)(k_rows - k0);
     } else {
       base = reinterpret_cast<const char*>(p) + (long long)first * ld + k0 * (long long)sizeof(T);
-      step = kKBytes;
+      step = kKBytes<T>;
       k_left = 0;
     }
 #pragma unroll
@@ -147,20 +169,24 @@ struct Loader {
           (__attribute__((address_space(3))) void*)(lds + instr * 1024), 16, 0, 0);
     }
     base += step;
-    if constexpr (ACROSS) k_left -= kKElems<T>;
+    if constexpr (ACROSS) k_left -= kKElems;
   }
 };
 
 // Fragment of 16 rows (or columns) from m0 on
 template <typename T, bool ACROSS, int N>
-__device__ inline Frag read_frag(const char* lds, int m0, int lane) {
-  Frag r;
+__device__ inline typename Elem<T>::Frag read_frag(const char* lds, int m0, int lane) {
+  typename Elem<T>::Frag r;
+  const int g = lane >> 4;
   if constexpr (!ACROSS) {
-    const int row = m0 + (lane & 15);
-    const int c = (lane >> 4) ^ swizzle<T, false, N>(row);
-    r.i = *reinterpret_cast<const i32x4*>(lds + row * kKBytes + c * 16);
+    const int row = m0 + (lane & 15), swz = swizzle<T, false, N>(row);
+    const char* at = lds + row * kKBytes<T>;
+    if constexpr (sizeof(T) == 2) r.i = *reinterpret_cast<const i32x4*>(at + (g ^ swz) * 16);
+    else
+#pragma unroll
+      for (int h = 0; h < 2; ++h) r.x[h] = *reinterpret_cast<const f32x4*>(at + ((4 * h + g) ^ swz) * 16);
   } else if constexpr (sizeof(T) == 2) {
-    const int g = lane >> 4, j = (lane & 15) >> 2, q = lane & 3;
+    const int j = (lane & 15) >> 2, q = lane & 3;
     const int chunk = m0 / 8 + (q >> 1);
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -171,11 +197,13 @@ __device__ inline Frag read_frag(const char* lds, int m0, int lane) {
   } else {
     const int col = m0 + (lane & 15);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int row = 4 * (lane >> 4) + i;
-      r.f[i] = *reinterpret_cast<const float*>(lds + row * (N * 4) + ((col / 4) ^ swizzle<T, true, N>(row)) * 16 +
-                                               (col & 3) * 4);
-    }
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int row = 16 * h + 4 * g + i;
+        r.x[h][i] = *reinterpret_cast<const float*>(lds + row * (N * 4) + ((col / 4) ^ swizzle<T, true, N>(row)) * 16 +
+                                                    (col & 3) * 4);
+      }
   }
   return r;
 }
@@ -193,9 +221,9 @@ struct Cfg {
   static constexpr int kThreads = WA * WB * 64;
   static constexpr int kWavesPerSimd = PER * WA * WB / 4;
   static constexpr int kSlots = 256 * PER;                 // blocks that run at once on 256 CUs
-  static constexpr int kStage = (BA + BB) * kKBytes;
-  static constexpr int kLds = S * kStage;
 };
+template <typename T, class C> constexpr int kStageBytes = (C::BA + C::BB) * kKBytes<T>;
+template <typename T, class C> constexpr int kLdsBytes = C::S * kStageBytes<T, C>;
 
 struct TileArgs {
   const void* hidden;     // packed rows (row_pad, dim_pad)
@@ -218,15 +246,15 @@ struct TileArgs {
   int mean;
 };
 
-// The id-th of `a_tiles` x `b_tiles` tiles, from column b_first on, of part `split` of `splits` of K.  smem: C::kLds bytes.
+// The id-th of `a_tiles` x `b_tiles` tiles, from column b_first on, of part `split` of `splits` of K.  smem: kLdsBytes.
 template <typename T, class C, int MODE>
 __device__ __forceinline__ void run_tile(const TileArgs& p, int count, int id, int a_tiles, int b_tiles, int b_first,
                                          int splits, char* smem) {
   constexpr bool kAAcross = MODE == kDhid || MODE == kDwei;
   constexpr bool kBAcross = MODE == kDwei;
-  constexpr int BA = C::BA, BB = C::BB, WA = C::WA, WB = C::WB, kStages = C::S, kStage = C::kStage;
+  constexpr int BA = C::BA, BB = C::BB, WA = C::WA, WB = C::WB, kStages = C::S, kStage = kStageBytes<T, C>;
   constexpr int NW = WA * WB, TA = BA / WA, TB = BB / WB, FA = TA / 16, FB = TB / 16;
-  constexpr int KE = kKElems<T>;
+  constexpr int KE = kKElems;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
 
   const int plane = a_tiles * b_tiles;
@@ -250,107 +278,137 @@ __device__ __forceinline__ void run_tile(const TileArgs& p, int count, int id, i
     k_tiles = min(each, all - k_first);
   }
 
-  Loader<T, kAAcross, BA, NW> la;
-  Loader<T, kBAcross, BB, NW> lb;
-  const T* weight = static_cast<const T*>(p.weight);
-  const T* prob = static_cast<const T*>(p.prob);
-  if constexpr (MODE == kStats || MODE == kProb) {
-    la.init(weight, p.weight_ld, a0, p.piece, 0, 0, wave, lane);
-    lb.init(static_cast<const T*>(p.hidden), p.dim_pad, b0, b0 + BB, 0, 0, wave, lane);
-  } else if constexpr (MODE == kDhid) {
-    la.init(weight, p.weight_ld, a0, p.dim_pad, (long long)k_first * KE, p.piece, wave, lane);
-    lb.init(prob, p.prob_ld, b0, b0 + BB, (long long)k_first * KE, 0, wave, lane);
-  } else {
-    la.init(static_cast<const T*>(p.weighted), p.dim_pad, a0, p.dim_pad, 0, p.row_pad, wave, lane);
-    lb.init(prob, p.prob_ld, b0, (int)p.prob_ld, 0, p.row_pad, wave, lane);
-  }
-
   const int wa = wave % WA, wb = wave / WA;
   f32x4 acc[FA][FB];
-#pragma unroll
-  for (int i = 0; i < FA; ++i)
-#pragma unroll
-    for (int j = 0; j < FB; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  auto product = [&](auto exact) {
+    Loader<T, kAAcross, BA, NW> la;
+    Loader<T, kBAcross, BB, NW> lb;
+    const T* weight = static_cast<const T*>(p.weight);
+    const T* prob = static_cast<const T*>(p.prob);
+    if constexpr (MODE == kStats || MODE == kProb) {
+      la.init(weight, p.weight_ld, a0, p.piece, 0, 0, wave, lane);
+      lb.init(static_cast<const T*>(p.hidden), p.dim_pad, b0, b0 + BB, 0, 0, wave, lane);
+    } else if constexpr (MODE == kDhid) {
+      la.init(weight, p.weight_ld, a0, p.dim_pad, (long long)k_first * KE, p.piece, wave, lane);
+      lb.init(prob, p.prob_ld, b0, b0 + BB, (long long)k_first * KE, 0, wave, lane);
+    } else {
+      la.init(static_cast<const T*>(p.weighted), p.dim_pad, a0, p.dim_pad, 0, p.row_pad, wave, lane);
+      lb.init(prob, p.prob_ld, b0, (int)p.prob_ld, 0, p.row_pad, wave, lane);
+    }
 
-  // kStages K tiles in LDS, all but one of them on their way while one is multiplied.  Per tile: wait until this wave's
-  // part of the oldest has arrived (the younger ones may stay under way), one barrier -- now everybody's has, and
-  // everybody has read the tile before it, whose place the next fetch takes -- then read fragments and multiply.
-  // (The barrier is written out: __syncthreads would wait for every fetch.)
-  constexpr int kFetches = decltype(la)::kPer + decltype(lb)::kPer;      // of every wave, per tile
-  auto fetch = [&](auto last, int stage) {
-    char* to = smem + stage * kStage;
-    la.template issue<decltype(last)::value>(to);
-    lb.template issue<decltype(last)::value>(to + BA * kKBytes);
-  };
-  Frag fa[FA], fb[FB];
-  auto read = [&](int stage) {
-    const char* sa = smem + stage * kStage;
-    const char* sb = sa + BA * kKBytes;
-#pragma unroll
-    for (int i = 0; i < FA; ++i) fa[i] = read_frag<T, kAAcross, BA>(sa, wa * TA + i * 16, lane);
-#pragma unroll
-    for (int j = 0; j < FB; ++j) fb[j] = read_frag<T, kBAcross, BB>(sb, wb * TB + j * 16, lane);
-  };
-  auto multiply = [&] {
 #pragma unroll
     for (int i = 0; i < FA; ++i)
 #pragma unroll
-      for (int j = 0; j < FB; ++j) acc[i][j] = Elem<T>::mma(fa[i], fb[j], acc[i][j]);
-  };
+      for (int j = 0; j < FB; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+    // kStages K tiles in LDS, all but one of them on their way while one is multiplied.  Per tile: wait until this wave's
+    // part of the oldest has arrived (the younger ones may stay under way), one barrier -- now everybody's has, and
+    // everybody has read the tile before it, whose place the next fetch takes -- then read fragments and multiply.
+    // (The barrier is written out: __syncthreads would wait for every fetch.)
+    constexpr int kFetches = decltype(la)::kPer + decltype(lb)::kPer;      // of every wave, per tile
+    auto fetch = [&](auto last, int stage) {
+      char* to = smem + stage * kStage;
+      la.template issue<decltype(last)::value>(to);
+      lb.template issue<decltype(last)::value>(to + BA * kKBytes<T>);
+    };
+    typename Elem<T>::Frag fa[FA], fb[FB];
+    auto read = [&](int stage) {
+      const char* sa = smem + stage * kStage;
+      const char* sb = sa + BA * kKBytes<T>;
 #pragma unroll
-  for (int t = 0; t < kStages - 1; ++t)
-    if (t < k_tiles) {
-      if (t + 1 < k_tiles) fetch(No{}, t);
-      else fetch(Yes{}, t);
-    }
-  int stage = 0, free = kStages - 1;
-  auto advance = [&] {
-    free = stage;
-    stage = stage + 1 == kStages ? 0 : stage + 1;
-  };
-  if constexpr (NW == 8) {
-    // Two waves per SIMD take turns: while one reads its fragments the other multiplies, one barrier per turn, the
-    // second group half a tile behind the first.
-    if (k_tiles >= kStages - 1) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((kStages - 2) * kFetches) : "memory");
-    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    asm volatile("s_barrier" ::: "memory");
-    const bool second = wave >= 4;
-    if (second) asm volatile("s_barrier" ::: "memory");
-    auto turn = [&](auto more) {
-      read(stage);
-      if constexpr (decltype(more)::value == 2) fetch(No{}, free);
-      if constexpr (decltype(more)::value == 1) fetch(Yes{}, free);
-      if constexpr (decltype(more)::value > 0)
-        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((kStages - 2) * kFetches) : "memory");
-      else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-      __builtin_amdgcn_sched_barrier(0);
-      __builtin_amdgcn_s_setprio(1);
-      multiply();
-      __builtin_amdgcn_s_setprio(0);
-      __builtin_amdgcn_sched_barrier(0);
+      for (int i = 0; i < FA; ++i) fa[i] = read_frag<T, kAAcross, BA>(sa, wa * TA + i * 16, lane);
+#pragma unroll
+      for (int j = 0; j < FB; ++j) fb[j] = read_frag<T, kBAcross, BB>(sb, wb * TB + j * 16, lane);
+    };
+    auto multiply = [&] {
+      if constexpr (sizeof(T) == 2) {
+#pragma unroll
+        for (int i = 0; i < FA; ++i)
+#pragma unroll
+          for (int j = 0; j < FB; ++j) acc[i][j] = Elem<T>::mma(fa[i], fb[j], acc[i][j]);
+      } else if constexpr (decltype(exact)::value) {
+#pragma unroll
+        for (int i = 0; i < FA; ++i)
+#pragma unroll
+          for (int j = 0; j < FB; ++j) acc[i][j] = Elem<T>::mma_exact(fa[i], fb[j], acc[i][j]);
+      } else {
+        typename Elem<T>::Parts pb[FB];
+#pragma unroll
+        for (int j = 0; j < FB; ++j) pb[j] = Elem<T>::split(fb[j]);
+#pragma unroll
+        for (int i = 0; i < FA; ++i) {
+          const auto pa = Elem<T>::split(fa[i]);
+#pragma unroll
+          for (int j = 0; j < FB; ++j) acc[i][j] = Elem<T>::mma(pa, pb[j], acc[i][j]);
+        }
+      }
+    };
+#pragma unroll
+    for (int t = 0; t < kStages - 1; ++t)
+      if (t < k_tiles) {
+        if (t + 1 < k_tiles) fetch(No{}, t);
+        else fetch(Yes{}, t);
+      }
+    int stage = 0, free = kStages - 1;
+    auto advance = [&] {
+      free = stage;
+      stage = stage + 1 == kStages ? 0 : stage + 1;
+    };
+    if constexpr (NW == 8) {
+      // Two waves per SIMD take turns: while one reads its fragments the other multiplies, one barrier per turn, the
+      // second group half a tile behind the first.
+      if (k_tiles >= kStages - 1) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((kStages - 2) * kFetches) : "memory");
+      else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
       asm volatile("s_barrier" ::: "memory");
-      advance();
-    };
-    int t = 0;
-    for (; t + kStages < k_tiles; ++t) turn(Const<2>{});
-    for (; t + kStages - 1 < k_tiles; ++t) turn(Const<1>{});
-    for (; t < k_tiles; ++t) turn(Const<0>{});
-    if (!second) asm volatile("s_barrier" ::: "memory");
-  } else {
-    auto tile = [&](auto more) {
-      if constexpr (decltype(more)::value > 0)
-        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((kStages - 2) * kFetches) : "memory");
-      else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-      if constexpr (decltype(more)::value == 2) fetch(No{}, free);
-      if constexpr (decltype(more)::value == 1) fetch(Yes{}, free);
-      read(stage);
-      multiply();
-      advance();
-    };
-    int t = 0;
-    for (; t + kStages < k_tiles; ++t) tile(Const<2>{});
-    for (; t + kStages - 1 < k_tiles; ++t) tile(Const<1>{});
-    for (; t < k_tiles; ++t) tile(Const<0>{});
+      const bool second = wave >= 4;
+      if (second) asm volatile("s_barrier" ::: "memory");
+      auto turn = [&](auto more) {
+        read(stage);
+        if constexpr (decltype(more)::value == 2) fetch(No{}, free);
+        if constexpr (decltype(more)::value == 1) fetch(Yes{}, free);
+        if constexpr (decltype(more)::value > 0)
+          asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((kStages - 2) * kFetches) : "memory");
+        else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        __builtin_amdgcn_sched_barrier(0);
+        __builtin_amdgcn_s_setprio(1);
+        multiply();
+        __builtin_amdgcn_s_setprio(0);
+        __builtin_amdgcn_sched_barrier(0);
+        asm volatile("s_barrier" ::: "memory");
+        advance();
+      };
+      int t = 0;
+      for (; t + kStages < k_tiles; ++t) turn(Const<2>{});
+      for (; t + kStages - 1 < k_tiles; ++t) turn(Const<1>{});
+      for (; t < k_tiles; ++t) turn(Const<0>{});
+      if (!second) asm volatile("s_barrier" ::: "memory");
+    } else {
+      auto tile = [&](auto more) {
+        if constexpr (decltype(more)::value > 0)
+          asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((kStages - 2) * kFetches) : "memory");
+        else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        if constexpr (decltype(more)::value == 2) fetch(No{}, free);
+        if constexpr (decltype(more)::value == 1) fetch(Yes{}, free);
+        read(stage);
+        multiply();
+        advance();
+      };
+      int t = 0;
+      for (; t + kStages < k_tiles; ++t) tile(Const<2>{});
+      for (; t + kStages - 1 < k_tiles; ++t) tile(Const<1>{});
+      for (; t < k_tiles; ++t) tile(Const<0>{});
+    }
+  };
+  product(No{});
+  if constexpr (sizeof(T) == 4) {
+    bool bad = false;
+#pragma unroll
+    for (int i = 0; i < FA; ++i)
+#pragma unroll
+      for (int j = 0; j < FB; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) bad |= acc[i][j][e] != acc[i][j][e];
+    if (__syncthreads_or(bad)) product(Yes{});
   }
 
   // acc[i][j][e] belongs to a = a0 + wa TA + 16 i + 4 (lane / 16) + e and b = b0 + wb TB + 16 j + lane % 16
@@ -485,13 +543,14 @@ __device__ inline int tile_of(int b, int tiles) {
 // same threads (552 rows as 2 x 256 + 64 instead of 3 x 256).
 template <class C>
 struct Strips {
-  static constexpr bool kNarrow = C::BB == 256;
-  using Half = Cfg<C::BA, kNarrow ? 128 : C::BB, C::WA, C::WB, C::S, C::PER>;
-  using Quarter = Cfg<C::BA, kNarrow ? 64 : C::BB, C::WA, C::WB, C::S, C::PER>;
-  int whole, rest;              // strips of C::BB rows; rows of the narrow strip: 0, 64 or 128
+  static constexpr bool kNarrow = C::BB >= 128;
+  static constexpr int kHalf = kNarrow ? C::BB / 2 : C::BB, kQuarter = kNarrow ? C::BB / 4 : C::BB;
+  using Half = Cfg<C::BA, kHalf, C::WA, C::WB, C::S, C::PER>;
+  using Quarter = Cfg<C::BA, kQuarter, C::WA, C::WB, C::S, C::PER>;
+  int whole, rest;              // strips of C::BB rows; rows of the narrow strip: 0, a quarter or half of that
   __device__ explicit Strips(int count) {
     const int over = count % C::BB;
-    rest = !kNarrow || over == 0 || over > 128 ? 0 : over > 64 ? 128 : 64;
+    rest = !kNarrow || over == 0 || over > kHalf ? 0 : over > kQuarter ? kHalf : kQuarter;
     whole = count / C::BB + (over > 0 && rest == 0);
   }
 };
@@ -513,7 +572,7 @@ __device__ __forceinline__ bool run_strips(const TileArgs& p, int count, int& b,
     if (b < run_blocks(narrow)) {
       const int id = tile_of(b, narrow);
       if (id >= 0) {
-        if (s.rest == 64) run_tile<T, typename S::Quarter, MODE>(p, count, id, a_tiles, 1, s.whole * C::BB, splits, smem);
+        if (s.rest == S::kQuarter) run_tile<T, typename S::Quarter, MODE>(p, count, id, a_tiles, 1, s.whole * C::BB, splits, smem);
         else run_tile<T, typename S::Half, MODE>(p, count, id, a_tiles, 1, s.whole * C::BB, splits, smem);
       }
       return true;
@@ -846,14 +905,10 @@ __global__ __launch_bounds__(256) void lce_dhid_kernel(const DhidArgs p) {
 
 // ---- host side ----------------------------------------------------------------------------------------------
 using Large = Cfg<256, 256, 4, 2, 4, 1>;
-using Medium = Cfg<256, 128, 2, 2, 3, 2>;
-using Fine = Cfg<128, 64, 2, 2, 4, 3>;         // float32, whose products take eight times as long per byte
+using Float = Cfg<128, 128, 2, 2, 2, 2>;
 using Small = Cfg<128, 32, 4, 1, 4, 4>;
+using SmallFloat = Cfg<128, 32, 4, 1, 3, 2>;
 constexpr int kStatsRows = 128;                // fewest vocabulary rows of a tile: room for the statistics
-#ifndef WFE_LR
-#define WFE_LR 192
-#endif
-constexpr int kLargeRows = WFE_LR;
 #ifndef WFE_PB
 #define WFE_PB 128
 #endif
@@ -862,10 +917,8 @@ constexpr long long kPieceBytes = (long long)WFE_PB << 20;     // most that the 
 // calls f with the tile that suits this many rows
 template <typename T, class F>
 hipError_t with_tile(int64_t rows, F f) {
-  if (rows <= Small::BB) return f(Small{});
-  if (rows > kLargeRows) return f(Large{});
-  if constexpr (sizeof(T) == 4) return f(Fine{});
-  else return f(Medium{});
+  if constexpr (sizeof(T) == 4) return rows <= SmallFloat::BB ? f(SmallFloat{}) : f(Float{});
+  else return rows <= Small::BB ? f(Small{}) : f(Large{});
 }
 
 long long up(long long x, long long to) { return (x + to - 1) / to * to; }
@@ -885,7 +938,7 @@ int tiles_of(long long x, bool a) { return (int)((x + (a ? C::BA : C::BB) - 1) /
 Plan make_plan(const wfe_linear_ce& d, const void* weight, bool backward, int grads) {
   Plan p{};
   p.size = d.dtype == WFE_F32 ? 4 : 2;
-  p.ke = kKBytes / p.size;
+  p.ke = kKElems;
   p.dim_pad = lce_dim_pad(d);
   p.row_pad = lce_row_pad(d);
   // in place: whole K tiles, 16-byte rows, offsets inside a tile in 32 bits
@@ -931,7 +984,7 @@ Plan make_plan(const wfe_linear_ce& d, const void* weight, bool backward, int gr
     if (e_ != hipSuccess) return e_;       \
   } while (0)
 
-template <auto KERNEL, class C, class A>
+template <typename T, auto KERNEL, class C, class A>
 hipError_t launch(const A& args, long long blocks, hipStream_t stream) {
   static unsigned long long done = 0;           // a bit per device: more than 64 KB of LDS has been asked for
   int device = 0;
@@ -939,11 +992,11 @@ hipError_t launch(const A& args, long long blocks, hipStream_t stream) {
   const unsigned long long bit = 1ull << (device & 63);
   if (!(__atomic_load_n(&done, __ATOMIC_RELAXED) & bit)) {
     LCE_TRY(hipFuncSetAttribute(reinterpret_cast<const void*>(KERNEL), hipFuncAttributeMaxDynamicSharedMemorySize,
-                                C::kLds));
+                                (kLdsBytes<T, C>)));
     __atomic_fetch_or(&done, bit, __ATOMIC_RELAXED);
   }
   if (blocks > 0x7ffffff0ll) return hipErrorInvalidValue;
-  KERNEL<<<dim3((unsigned)blocks), dim3(C::kThreads), C::kLds, stream>>>(args);
+  KERNEL<<<dim3((unsigned)blocks), dim3(C::kThreads), kLdsBytes<T, C>, stream>>>(args);
   return hipGetLastError();
 }
 
@@ -980,7 +1033,7 @@ template <typename T, class C>
 hipError_t stats(const wfe_linear_ce& d, const TileArgs& a, int* tiles, hipStream_t stream) {
   static_assert(C::BA >= kStatsRows, "room for the statistics");
   *tiles = tiles_of<C>(d.vocab, true);
-  return launch<lce_logits_kernel<T, C, kStats>, C>(a, strip_blocks<C>(*tiles, d.rows), stream);
+  return launch<T, lce_logits_kernel<T, C, kStats>, C>(a, strip_blocks<C>(*tiles, d.rows), stream);
 }
 
 template <typename T>
@@ -1053,7 +1106,7 @@ hipError_t gradients(const wfe_linear_ce& d, const Plan& p, GradArgs& g, char* w
       a.v0 = 0;
       a.piece = g.next_piece;
       a.prob = g.next_prob;
-      LCE_TRY((launch<lce_logits_kernel<T, C, kProb>, C>(a, strip_blocks<C>(a_tiles, d.rows), stream)));
+      LCE_TRY((launch<T, lce_logits_kernel<T, C, kProb>, C>(a, strip_blocks<C>(a_tiles, d.rows), stream)));
       continue;
     }
     g.t.v0 = v0;
@@ -1064,7 +1117,7 @@ hipError_t gradients(const wfe_linear_ce& d, const Plan& p, GradArgs& g, char* w
     const long long blocks = (g.dwei ? up((long long)g.rule.dim_tiles * tiles_of<C>(g.t.piece, false), 8) : 0) +
                              (g.dhid ? strip_blocks<C>((long long)g.rule.dim_tiles * p.splits, d.rows) : 0) +
                              (g.next_piece > 0 ? strip_blocks<C>(a_tiles, d.rows) : 0);
-    if (blocks > 0) LCE_TRY((launch<lce_grads_kernel<T, C>, C>(g, blocks, stream)));
+    if (blocks > 0) LCE_TRY((launch<T, lce_grads_kernel<T, C>, C>(g, blocks, stream)));
   }
   return hipSuccess;
 }
