@@ -94,24 +94,24 @@ __device__ inline float exp_of(float x) { return __builtin_amdgcn_exp2f(x * kLog
 // An operand tile in LDS is either rows x 32 of K ("along": K contiguous in memory) or K rows x columns
 // ("across": K strided in memory, transposed by the read).  16-byte chunks of a row are permuted by an exclusive or
 // so that the lanes of a fragment read meet different banks:
-//   along, 2 byte   rows of 4 chunks, 4 rows cover the banks: rows 4 apart take different pairs of chunks (a 16-byte
+//   along, 64 bytes rows of 4 chunks, 4 rows cover the banks: rows 4 apart take different pairs of chunks (a 16-byte
 //                   read serves 8 lanes of one chunk number with 8 of the next at a time)
-//   along, 4 byte   rows of 8 chunks: chunk ^ (row & 7)
+//   along, 128      rows of 8 chunks: chunk ^ (row & 7)
 //   across, 2 byte  pairs of chunks (a transposing read takes 32 bytes of each of 4 rows); 8 rows 0..3, 8..11 apart
 //   across, 4 byte  groups of four chunks; 4 rows 4 apart
-template <typename T, bool ACROSS, int N>
+template <typename T, bool ACROSS, int N, int KS>
 __device__ inline int swizzle(int row) {
-  if constexpr (!ACROSS) return sizeof(T) == 2 ? (row >> 1) & 2 : row & 7;
+  if constexpr (!ACROSS) return KS * sizeof(T) == 2 ? (row >> 1) & 2 : row & 7;
   else if constexpr (sizeof(T) == 2) return (((row & 3) | ((row >> 1) & 4)) & (N / 16 - 1)) << 1;
   else return (((row >> 2) & 3) & (N / 16 - 1)) << 2;
 }
 
 // Loads tiles of N rows (or columns) with NW waves, 1024 bytes per wave and instruction straight into LDS.
-template <typename T, bool ACROSS, int N, int NW>
+template <typename T, bool ACROSS, int N, int NW, int KS>
 struct Loader {
-  static constexpr int kRowBytes = ACROSS ? N * (int)sizeof(T) : kKBytes<T>;
+  static constexpr int kRowBytes = ACROSS ? N * (int)sizeof(T) : KS * kKBytes<T>;
   static constexpr int kChunks = kRowBytes / 16;
-  static constexpr int kTileBytes = N * kKBytes<T>;
+  static constexpr int kTileBytes = N * KS * kKBytes<T>;
   static constexpr int kInstrs = kTileBytes / 1024;
   static constexpr int kPer = (kInstrs + NW - 1) / NW;
   const char* base;
@@ -130,18 +130,18 @@ struct Loader {
     ld = ld_elems * (long long)sizeof(T);
     if constexpr (ACROSS) {
       base = reinterpret_cast<const char*>(p) + k0 * ld + (long long)first * sizeof(T);
-      step = ld * kKElems;
+      step = ld * kKElems * KS;
       k_left = (int)(k_rows - k0);
     } else {
       base = reinterpret_cast<const char*>(p) + (long long)first * ld + k0 * (long long)sizeof(T);
-      step = kKBytes<T>;
+      step = KS * kKBytes<T>;
       k_left = 0;
     }
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
       const int id = (i * NW + wave) % kInstrs * 64 + lane;     // (a small tile: some waves fetch the same again)
       int row = id / kChunks;
-      int c = (id % kChunks) ^ swizzle<T, ACROSS, N>(row);
+      int c = (id % kChunks) ^ swizzle<T, ACROSS, N, KS>(row);
       if constexpr (ACROSS) {
         const int most = (int)((limit - first) * (int)sizeof(T) / 16) - 1;
         c = c < most ? c : most;          // columns past the end: any that exist, their products are not stored
@@ -169,30 +169,30 @@ struct Loader {
           (__attribute__((address_space(3))) void*)(lds + instr * 1024), 16, 0, 0);
     }
     base += step;
-    if constexpr (ACROSS) k_left -= kKElems;
+    if constexpr (ACROSS) k_left -= KS * kKElems;
   }
 };
 
-// Fragment of 16 rows (or columns) from m0 on
-template <typename T, bool ACROSS, int N>
-__device__ inline typename Elem<T>::Frag read_frag(const char* lds, int m0, int lane) {
+// Fragment of 16 rows (or columns) from m0 on, step ks of the tile's KS
+template <typename T, bool ACROSS, int N, int KS>
+__device__ inline typename Elem<T>::Frag read_frag(const char* lds, int m0, int ks, int lane) {
   typename Elem<T>::Frag r;
   const int g = lane >> 4;
   if constexpr (!ACROSS) {
-    const int row = m0 + (lane & 15), swz = swizzle<T, false, N>(row);
-    const char* at = lds + row * kKBytes<T>;
-    if constexpr (sizeof(T) == 2) r.i = *reinterpret_cast<const i32x4*>(at + (g ^ swz) * 16);
+    const int row = m0 + (lane & 15), swz = swizzle<T, false, N, KS>(row);
+    const char* at = lds + row * (KS * kKBytes<T>);
+    if constexpr (sizeof(T) == 2) r.i = *reinterpret_cast<const i32x4*>(at + ((4 * ks + g) ^ swz) * 16);
     else
 #pragma unroll
-      for (int h = 0; h < 2; ++h) r.x[h] = *reinterpret_cast<const f32x4*>(at + ((4 * h + g) ^ swz) * 16);
+      for (int h = 0; h < 2; ++h) r.x[h] = *reinterpret_cast<const f32x4*>(at + ((8 * ks + 4 * h + g) ^ swz) * 16);
   } else if constexpr (sizeof(T) == 2) {
     const int j = (lane & 15) >> 2, q = lane & 3;
     const int chunk = m0 / 8 + (q >> 1);
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const int row = 8 * g + 4 * h + j;
+      const int row = 32 * ks + 8 * g + 4 * h + j;
       r.s[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(
-          lds + row * (N * 2) + (chunk ^ swizzle<T, true, N>(row)) * 16 + (q & 1) * 8));
+          lds + row * (N * 2) + (chunk ^ swizzle<T, true, N, KS>(row)) * 16 + (q & 1) * 8));
     }
   } else {
     const int col = m0 + (lane & 15);
@@ -200,8 +200,8 @@ __device__ inline typename Elem<T>::Frag read_frag(const char* lds, int m0, int 
     for (int h = 0; h < 2; ++h)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int row = 16 * h + 4 * g + i;
-        r.x[h][i] = *reinterpret_cast<const float*>(lds + row * (N * 4) + ((col / 4) ^ swizzle<T, true, N>(row)) * 16 +
+        const int row = 32 * ks + 16 * h + 4 * g + i;
+        r.x[h][i] = *reinterpret_cast<const float*>(lds + row * (N * 4) + ((col / 4) ^ swizzle<T, true, N, KS>(row)) * 16 +
                                                     (col & 3) * 4);
       }
   }
@@ -214,15 +214,15 @@ struct Yes { static constexpr bool value = true; };
 struct No { static constexpr bool value = false; };
 enum Mode { kStats, kProb, kDhid, kDwei };
 
-// A block's tile: BA x BB results of WA x WB waves, S K tiles in LDS, PER blocks on a CU at a time
-template <int BA_, int BB_, int WA_, int WB_, int S_, int PER_>
+// A block's tile: BA x BB results of WA x WB waves, S K tiles of KS steps of 32 in LDS, PER blocks on a CU at a time
+template <int BA_, int BB_, int WA_, int WB_, int S_, int PER_, int KS_ = 1>
 struct Cfg {
-  static constexpr int BA = BA_, BB = BB_, WA = WA_, WB = WB_, S = S_, PER = PER_;
+  static constexpr int BA = BA_, BB = BB_, WA = WA_, WB = WB_, S = S_, PER = PER_, KS = KS_;
   static constexpr int kThreads = WA * WB * 64;
   static constexpr int kWavesPerSimd = PER * WA * WB / 4;
   static constexpr int kSlots = 256 * PER;                 // blocks that run at once on 256 CUs
 };
-template <typename T, class C> constexpr int kStageBytes = (C::BA + C::BB) * kKBytes<T>;
+template <typename T, class C> constexpr int kStageBytes = (C::BA + C::BB) * C::KS * kKBytes<T>;
 template <typename T, class C> constexpr int kLdsBytes = C::S * kStageBytes<T, C>;
 
 struct TileArgs {
@@ -252,9 +252,9 @@ __device__ __forceinline__ void run_tile(const TileArgs& p, int count, int id, i
                                          int splits, char* smem) {
   constexpr bool kAAcross = MODE == kDhid || MODE == kDwei;
   constexpr bool kBAcross = MODE == kDwei;
-  constexpr int BA = C::BA, BB = C::BB, WA = C::WA, WB = C::WB, kStages = C::S, kStage = kStageBytes<T, C>;
+  constexpr int BA = C::BA, BB = C::BB, WA = C::WA, WB = C::WB, kStages = C::S, kStage = kStageBytes<T, C>, KS = C::KS;
   constexpr int NW = WA * WB, TA = BA / WA, TB = BB / WB, FA = TA / 16, FB = TB / 16;
-  constexpr int KE = kKElems;
+  constexpr int KE = kKElems * KS;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
 
   const int plane = a_tiles * b_tiles;
@@ -281,8 +281,8 @@ __device__ __forceinline__ void run_tile(const TileArgs& p, int count, int id, i
   const int wa = wave % WA, wb = wave / WA;
   f32x4 acc[FA][FB];
   auto product = [&](auto exact) {
-    Loader<T, kAAcross, BA, NW> la;
-    Loader<T, kBAcross, BB, NW> lb;
+    Loader<T, kAAcross, BA, NW, KS> la;
+    Loader<T, kBAcross, BB, NW, KS> lb;
     const T* weight = static_cast<const T*>(p.weight);
     const T* prob = static_cast<const T*>(p.prob);
     if constexpr (MODE == kStats || MODE == kProb) {
@@ -309,16 +309,16 @@ __device__ __forceinline__ void run_tile(const TileArgs& p, int count, int id, i
     auto fetch = [&](auto last, int stage) {
       char* to = smem + stage * kStage;
       la.template issue<decltype(last)::value>(to);
-      lb.template issue<decltype(last)::value>(to + BA * kKBytes<T>);
+      lb.template issue<decltype(last)::value>(to + BA * KS * kKBytes<T>);
     };
     typename Elem<T>::Frag fa[FA], fb[FB];
-    auto read = [&](int stage) {
+    auto read = [&](int stage, int ks) {
       const char* sa = smem + stage * kStage;
-      const char* sb = sa + BA * kKBytes<T>;
+      const char* sb = sa + BA * KS * kKBytes<T>;
 #pragma unroll
-      for (int i = 0; i < FA; ++i) fa[i] = read_frag<T, kAAcross, BA>(sa, wa * TA + i * 16, lane);
+      for (int i = 0; i < FA; ++i) fa[i] = read_frag<T, kAAcross, BA, KS>(sa, wa * TA + i * 16, ks, lane);
 #pragma unroll
-      for (int j = 0; j < FB; ++j) fb[j] = read_frag<T, kBAcross, BB>(sb, wb * TB + j * 16, lane);
+      for (int j = 0; j < FB; ++j) fb[j] = read_frag<T, kBAcross, BB, KS>(sb, wb * TB + j * 16, ks, lane);
     };
     auto multiply = [&] {
       if constexpr (sizeof(T) == 2) {
@@ -363,7 +363,8 @@ __device__ __forceinline__ void run_tile(const TileArgs& p, int count, int id, i
       const bool second = wave >= 4;
       if (second) asm volatile("s_barrier" ::: "memory");
       auto turn = [&](auto more) {
-        read(stage);
+        static_assert(KS == 1, "a turn is one step");
+        read(stage, 0);
         if constexpr (decltype(more)::value == 2) fetch(No{}, free);
         if constexpr (decltype(more)::value == 1) fetch(Yes{}, free);
         if constexpr (decltype(more)::value > 0)
@@ -389,8 +390,11 @@ __device__ __forceinline__ void run_tile(const TileArgs& p, int count, int id, i
         else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
         if constexpr (decltype(more)::value == 2) fetch(No{}, free);
         if constexpr (decltype(more)::value == 1) fetch(Yes{}, free);
-        read(stage);
-        multiply();
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+          read(stage, ks);
+          multiply();
+        }
         advance();
       };
       int t = 0;
@@ -907,6 +911,9 @@ __global__ __launch_bounds__(256) void lce_dhid_kernel(const DhidArgs p) {
 using Large = Cfg<256, 256, 4, 2, 4, 1>;
 using Float = Cfg<128, 128, 2, 2, 2, 2>;
 using Small = Cfg<128, 32, 4, 1, 4, 4>;
+// the statistics of few rows: W comes from memory once, in 128-byte pieces of its rows (16 x 1280 x 51866 fp16: 29 us; 64-byte
+// pieces 35)
+using Stream = Cfg<128, 32, 4, 1, 3, 2, 2>;
 using SmallFloat = Cfg<128, 32, 4, 1, 3, 2>;
 constexpr int kStatsRows = 128;                // fewest vocabulary rows of a tile: room for the statistics
 #ifndef WFE_PB
@@ -1070,7 +1077,8 @@ hipError_t forward(const wfe_linear_ce& d, const void* hidden, const void* weigh
   a.partial = reinterpret_cast<float2*>(ws + p.partial);
   int tiles = 0;
   if (d.rows > 0) {
-    LCE_TRY(with_tile<T>(d.rows, [&](auto c) { return stats<T, decltype(c)>(d, a, &tiles, stream); }));
+    if (sizeof(T) == 2 && d.rows <= Stream::BB) LCE_TRY((stats<T, Stream>(d, a, &tiles, stream)));
+    else LCE_TRY(with_tile<T>(d.rows, [&](auto c) { return stats<T, decltype(c)>(d, a, &tiles, stream); }));
   }
   float* row_loss = reinterpret_cast<float*>(ws + p.row_loss);
   float* total = none ? nullptr : loss;
@@ -1084,6 +1092,8 @@ hipError_t forward(const wfe_linear_ce& d, const void* hidden, const void* weigh
 
 template <typename T, class C>
 hipError_t gradients(const wfe_linear_ce& d, const Plan& p, GradArgs& g, char* ws, hipStream_t stream) {
+  // DWEI reads whole K tiles of rows, which PROB's narrowest strip has to have written
+  static_assert(C::KS * kKElems <= (Strips<C>::kNarrow ? Strips<C>::kQuarter : C::BB), "rows of d");
   const char* w = static_cast<const char*>(g.t.weight);
   g.rule.dim_tiles = tiles_of<C>(p.dim_pad, true);
   g.rule.bb = C::BB;
