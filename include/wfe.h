@@ -224,8 +224,8 @@ int wfe_power_spectrum(wfe_handle h, const float* wav, const int64_t* offsets, c
 
 /* ---- the decoder's vocabulary matrix ----------------------------------------- */
 /* The two operators at the ends of the decoder, where the collator's labels meet the vocabulary matrix W
- * (vocab, dim): the loss of WhisperForConditionalGeneration (proj_out and the cross entropy, as the Trainer of
- * finetune.py:143 / finetune_all.py calls it) and the embedding of its input tokens.
+ * (vocab, dim): the loss of WhisperForConditionalGeneration (proj_out and the cross entropy, as the
+ * Seq2SeqTrainer of finetune.py:144-150 calls it) and the embedding of its input tokens.
  * They take no handle: every call names its device and gets its workspace from the caller, so that calls on
  * different streams, from different threads or in different captured graphs share nothing.  Errors: a negative
  * wfe_status, its text in wfe_last_error(NULL) of the same thread.  Nothing is allocated, nothing synchronises,
@@ -237,7 +237,7 @@ typedef enum { WFE_REDUCE_NONE = 0, WFE_REDUCE_SUM = 1, WFE_REDUCE_MEAN = 2 } wf
 
 /* Softmax cross entropy of labels under logits = hidden @ W^T, the logits never kept:
  *   loss_n = log sum_v exp(h_n . W_v) - h_n . W_{y_n}     (0 where y_n == ignore_index, whatever h_n holds)
- * computed with float32 logits and sums.  A label outside 0..vocab-1 that is not ignore_index makes the loss NaN.
+ * computed with float32 logits and sums (float32 inputs: products exact to 2^-26 of themselves).  A label outside 0..vocab-1 that is not ignore_index makes the loss NaN.
  * Hidden row n lies at hidden + (n / inner) * outer_stride + (n % inner) * inner_stride (elements), so that a
  * (batch, length, dim) view is taken as it is; rows of W at weight + v * weight_stride.  dim is contiguous. */
 typedef struct {

@@ -139,6 +139,14 @@ def test_install_refuses_what_it_does_not_know_and_leaves_a_cpu_model_alone():
     feats, labels = torch.randn(2, 8, 20), torch.randint(0, 100, (2, 5))
     a, b = (m(input_features=feats, labels=labels) for m in (stock, model))
     assert torch.equal(a.loss, b.loss) and torch.equal(a.logits, b.logits)
+    import pickle
+    again = pickle.loads(pickle.dumps(model.get_output_embeddings()))
+    assert torch.equal(again(torch.ones(1, 16)), stock.get_output_embeddings()(torch.ones(1, 16)))
+    assert type(model).__name__ == type(stock).__name__ and decoder.install(model) is model
+    hooked = copy.deepcopy(stock)
+    hooked.forward = hooked.forward
+    with pytest.raises(ValueError, match="replaced already"):
+        decoder.install(hooked)
     odd = copy.deepcopy(stock)
     odd.set_output_embeddings(torch.nn.Linear(16, 103, bias=True))
     with pytest.raises(ValueError, match="not a plain one"):
@@ -158,7 +166,7 @@ def test_launcher_installs_the_operators_on_request(tmp_path, monkeypatch):
     script = tmp_path / "script.py"
     script.write_text("import os, transformers\n"
                       "m = transformers.WhisperForConditionalGeneration.from_pretrained(os.environ['MODEL_DIR'])\n"
-                      "open(os.environ['MODEL_DIR'] + '/seen', 'w').write(str(getattr(m, '_wfe_decoder', False)))\n")
+                      "open(os.environ['MODEL_DIR'] + '/seen', 'w').write(str(hasattr(m, 'wfe_logits_in_eval')))\n")
     monkeypatch.setenv("MODEL_DIR", str(tmp_path / "model"))
     before = WhisperForConditionalGeneration.__dict__.get("from_pretrained")
     try:

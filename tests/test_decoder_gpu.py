@@ -359,6 +359,159 @@ def test_two_calls_at_once_share_nothing():
         assert all(torch.equal(w, g) for g in gs)
 
 
+# rows around every strip and tile edge; vocabularies around the tiles'
+@pytest.mark.parametrize("dtype", [BF16, F16, F32], ids=["bf16", "f16", "f32"])
+@pytest.mark.parametrize("rows", [31, 32, 33, 63, 64, 65, 96, 97, 128, 160, 192, 255, 256, 257, 320, 321, 384, 385, 512])
+def test_every_row_kept_at_tile_edges(rows, dtype):
+    for vocab, dim in ((255, 64), (512, 192), (769, 96)):
+        h, w, y = make(rows, dim, vocab, dtype, seed=rows, ignored=0.0)
+        check(h, w, y, "sum")
+        check(h, w, y, "none")
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32], ids=["bf16", "f16", "f32"])
+def test_infinite_weights(dtype):
+    """Products with infinities follow float32: -inf logits drop out of the softmax, other rows stay exact."""
+    h, w, y = make(40, 64, 500, dtype, ignored=0.0)
+    y[y == 17] = 18
+    h[:, 0] = 1.0
+    clean = w.clone()
+    w[17, 0] = -float("inf")
+    loss = decoder().linear_cross_entropy(h, w, y, reduction="none")
+    z = h.double() @ clean.double().T
+    z[:, 17] = -float("inf")
+    want = torch.logsumexp(z, 1) - z.gather(1, y[:, None])[:, 0]
+    assert float((loss.double() - want).abs().max()) < 2e-5 * max(1.0, float(want.max()))
+    w[17, 0] = float("inf")
+    assert bool(torch.isnan(decoder().linear_cross_entropy(h, w, y, reduction="none")).all())
+
+
+def test_differentiable_once_and_again_on_the_same_graph():
+    d = decoder()
+    h, w, y = make(70, 64, 300, F32)
+    ids = y.clamp_min(0)
+    a, b = h.requires_grad_(), w.requires_grad_()
+    for out, of in ((d.linear_cross_entropy(a, b, y), (a, b)), (d.token_embedding(ids, b).sum(), (b,))):
+        first = torch.autograd.grad(out, of, retain_graph=True)
+        again = torch.autograd.grad(out, of, create_graph=True)
+        for x, z in zip(first, again):
+            assert torch.equal(x, z)
+        with pytest.raises(RuntimeError):                              # no path from the gradient to its input
+            torch.autograd.grad(again[-1].sum(), of, retain_graph=True)
+        with pytest.raises(RuntimeError, match="differentiated once"):
+            again[-1].sum().backward()
+
+
+def test_hidden_off_its_alignment_and_weights_with_strides():
+    g = torch.Generator(device="cuda").manual_seed(6)
+    for dtype in (BF16, F32):
+        base = torch.randn(50, 200, generator=g, device="cuda").to(dtype)
+        w = (torch.randn(333, 130, generator=g, device="cuda") / 11).to(dtype)
+        y = torch.randint(0, 333, (50,), generator=g, device="cuda")
+        check(base[:, 1:129], w[:, 1:129], y, "mean")                 # both off 16 bytes
+        check(base[:, 8:136], w[:, :128], y, "none")                  # rows of W 130 apart
+        check(base[:, 8:72].flip(0), w[1:2, :64].expand(333, 64), y, "sum", grads=(True, False))
+        check(base[:, 8:136][::2], w[::3, :128], y[::2] % 111, "mean")
+
+
+def test_two_captured_graphs_share_a_pool_and_threads_share_nothing():
+    import threading
+    d = decoder()
+    cases = [[t.requires_grad_() if t.is_floating_point() else t for t in make(n, 128, 1111, BF16, seed=n)] for n in (90, 400)]
+
+    def step(h, w, y):
+        loss = d.linear_cross_entropy(h, w, y)
+        return (loss.detach(), *torch.autograd.grad(loss, (h, w)))
+    want = [[t.clone() for t in step(*c)] for c in cases]
+    graphs = [torch.cuda.CUDAGraph() for _ in cases]
+    outs = []
+    for i, (graph, c) in enumerate(zip(graphs, cases)):
+        with torch.cuda.graph(graph, pool=graphs[0].pool() if i else None):
+            outs.append(step(*c))
+    for i in (0, 1, 1, 0, 1):
+        graphs[i].replay()
+        torch.cuda.synchronize()
+        for a, b in zip(outs[i], want[i]):
+            assert torch.equal(a, b)
+    got, errors = [None, None], []
+
+    def work(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(8):
+                    got[i] = step(*cases[i])
+                torch.cuda.current_stream().synchronize()
+        except Exception as e:  # noqa: BLE001 -- reported below
+            errors.append(e)
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors
+    for g, w in zip(got, want):
+        assert all(torch.equal(a, b) for a, b in zip(g, w))
+
+
+def test_offsets_past_32_bits():
+    """W of 4.5 GB and hidden states of 4.5 GB: addresses behind 2^32 bytes; spot checks against float64."""
+    d = decoder()
+    vocab, dim = 2_200_000, 1024
+    w = torch.empty(vocab, dim, device="cuda", dtype=BF16).normal_(0, 0.03)
+    y = torch.tensor([vocab - 1, 5, vocab // 2, vocab - 300, -100], device="cuda")
+    h = torch.randn(5, dim, device="cuda").to(BF16)
+    a, b = h.clone().requires_grad_(), w.requires_grad_()
+    loss = d.linear_cross_entropy(a, b, y, reduction="sum")
+    ga, gb = torch.autograd.grad(loss, (a, b))
+    z = torch.cat([h[:4].double() @ part.T.double() for part in w.detach().split(1 << 18)], dim=1)
+    logp = torch.log_softmax(z, 1)
+    want = -logp.gather(1, y[:4, None]).sum()
+    assert abs(float(loss) - float(want)) < 1e-4 * float(want)
+    p = logp.exp()
+    p[torch.arange(4), y[:4]] -= 1
+    for rows in (slice(vocab - 400, vocab), slice(0, 300), slice(1 << 21, (1 << 21) + 9)):
+        ref = p[:, rows].T @ h[:4].double()
+        assert float((gb[rows].double() - ref).abs().max()) < 0.02 * float(ref.abs().max()) + 1e-9
+    ref = sum(p[:, at:at + part.shape[0]] @ part.double() for at, part in
+              zip(range(0, vocab, 1 << 18), w.detach().split(1 << 18)))
+    assert float((ga[:4].double() - ref).abs().max()) < 0.02 * float(ref.abs().max())
+    ids = torch.tensor([vocab - 1, 0, vocab - 2, vocab - 1], device="cuda")
+    out = d.token_embedding(ids, b)
+    assert torch.equal(out, w.detach()[ids])
+    up = torch.randn(4, dim, device="cuda").to(BF16)
+    grad, = torch.autograd.grad(out, b, up)
+    assert torch.equal(grad[vocab - 2], up[2]) and torch.equal(grad[vocab - 1], (up[0].float() + up[3].float()).to(BF16))
+    assert not bool(grad[1:vocab - 2].any())
+    del w, b, gb, grad, z, logp, p, out
+    rows, vocab = 2_200_000, 257
+    h = torch.empty(rows, dim, device="cuda", dtype=BF16).normal_()
+    w = torch.randn(vocab, dim, device="cuda").mul_(0.03).to(BF16)
+    y = torch.randint(0, vocab, (rows,), device="cuda")
+    y[::7] = -100
+    a, b = h.requires_grad_(), w.requires_grad_()
+    loss = d.linear_cross_entropy(a, b, y, reduction="none")
+    ga, = torch.autograd.grad(loss, a, torch.ones_like(loss))
+    for part in (slice(0, 500), slice(rows - 700, rows), slice(1 << 21, (1 << 21) + 100)):
+        keep = y[part] != -100
+        z = h.detach()[part].double() @ w.detach().double().T
+        logp = torch.log_softmax(z, 1)
+        t = y[part].clamp_min(0)
+        ref = torch.where(keep, -logp.gather(1, t[:, None])[:, 0], 0.0)
+        assert float((loss[part].double() - ref).abs().max()) < 1e-3
+        p = logp.exp()
+        p[torch.arange(t.numel()), t] -= 1
+        ref = (p * keep[:, None]) @ w.detach().double()
+        assert float((ga[part].double() - ref).abs().max()) < 0.02 * float(ref.abs().max())
+    del ga, loss
+    up = h.detach()
+    ids = y.clamp_min(0)
+    grad, = torch.autograd.grad(d.token_embedding(ids, b), b, up)
+    ref = torch.zeros(vocab, dim, device="cuda", dtype=torch.float64)
+    for part, i in zip(up.split(1 << 18), ids.split(1 << 18)):
+        ref.index_add_(0, i, part.double())
+    assert float((grad.double() - ref).abs().max()) < 0.01 * float(ref.abs().max())
+
+
 # ---- embedding ---------------------------------------------------------------------------------------------
 def tokens(rows, vocab, seed=0, heavy=0.0):
     g = torch.Generator(device="cuda").manual_seed(seed)

@@ -123,11 +123,13 @@ void check_capture(const char* name, std::initializer_list<Tensor> inputs) {
     if (!node) continue;
     const auto made_on = node->stream();
     const auto stream = stream_of(t);
+    if (!made_on || made_on->id() == stream.id()) continue;
     hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
-    if (!made_on || made_on->id() == stream.id() ||
-        hipStreamIsCapturing(static_cast<hipStream_t>(raw(stream)), &status) != hipSuccess ||
-        status == hipStreamCaptureStatusNone)
+    if (hipStreamIsCapturing(static_cast<hipStream_t>(raw(stream)), &status) != hipSuccess) {
+      (void)hipGetLastError();
       continue;
+    }
+    if (status == hipStreamCaptureStatusNone) continue;
     throw std::runtime_error(std::string(name) + ": captured while the autograd graph of an earlier call with the same "
                              "parameter is alive; drop that call's results (or detach them) before capturing");
   }
@@ -135,7 +137,9 @@ void check_capture(const char* name, std::initializer_list<Tensor> inputs) {
 
 // Gradients that come from kernels cannot be differentiated again
 variable_list once(const char* name, variable_list grads) {
-  if (!at::GradMode::is_enabled()) return grads;
+  if (!at::GradMode::is_enabled()) return grads;           // create_graph was not asked for
+  for (Tensor& g : grads)
+    if (g.defined()) g = g.detach().set_requires_grad(true);
   return torch::autograd::DelayedError(std::string(name) + " can be differentiated once only", (int64_t)grads.size())
       .apply(std::move(grads));
 }

@@ -4,8 +4,7 @@
 * ``linear_cross_entropy`` the loss of the labels under ``hidden @ W.T`` without the logits ever being kept, and the
   gradients of ``hidden`` and W;
 * ``install``              puts both into a ``WhisperForConditionalGeneration``, whose training step
-  (finetune.py:143-153, finetune_all.py:143-153: the Trainer calls ``model(**batch)`` with the collator's labels) then
-  runs on them.
+  (the Seq2SeqTrainer of finetune.py:144-150 calls ``model(**batch)`` with the collator's labels) then runs on them.
 
 They work on the current stream of the tensors' device, allocate their workspace from torch's allocator and never
 synchronise, so they can be captured into a graph (not while the graph of an earlier call over the same parameters is
@@ -18,7 +17,6 @@ from __future__ import annotations
 import ctypes as C
 import functools
 import os
-import types
 from typing import Optional
 
 import torch
@@ -74,64 +72,84 @@ def token_embedding(ids: torch.Tensor, weight: torch.Tensor, *, scale: float = 1
 
 
 # ---- a Whisper model on them -------------------------------------------------------------------------------
-def _stock(module):
-    """The module's forward as a function of (module, ...): its class's, so that copies of the module keep working, or
-    the one that hooks have put into the instance."""
-    own = module.__dict__.get("forward")
-    return type(module).forward if own is None else lambda self, *args, **kwargs: own(*args, **kwargs)
+_TYPES = (torch.float32, torch.float16, torch.bfloat16)
+
+
+def _fits(weight: torch.Tensor) -> bool:
+    return weight.is_cuda and weight.dtype in _TYPES
+
+
+class _Embedding(torch.nn.Embedding):
+    def forward(self, ids):
+        if not _fits(self.weight):
+            return super().forward(ids)
+        return token_embedding(ids, self.weight, padding_idx=self.padding_idx)
+
+
+class _Head(torch.nn.Linear):
+    pass_hidden = False                         # a call wants the head's input instead of the logits
+
+    def forward(self, hidden):
+        return hidden if self.pass_hidden else super().forward(hidden)
+
+
+@functools.lru_cache(maxsize=None)
+def _model_class():
+    from transformers import WhisperForConditionalGeneration
+    from transformers.models.whisper.modeling_whisper import shift_tokens_right
+
+    class Model(WhisperForConditionalGeneration):
+        wfe_logits_in_eval = True
+
+        @functools.wraps(WhisperForConditionalGeneration.forward)
+        def forward(self, *args, **kwargs):
+            labels, head = kwargs.get("labels"), self.get_output_embeddings()
+            fused = labels is not None and _fits(head.weight) and (self.training or not self.wfe_logits_in_eval)
+            if not fused or kwargs.get("return_dict") is False:
+                return super().forward(*args, **kwargs)
+            if labels.shape[1] > self.max_target_positions:
+                raise ValueError(f"labels of {labels.shape[1]} tokens are longer than max_target_positions "
+                                 f"({self.max_target_positions})")
+            kwargs["labels"] = None
+            if kwargs.get("decoder_input_ids") is None and kwargs.get("decoder_inputs_embeds") is None:
+                kwargs["decoder_input_ids"] = shift_tokens_right(labels, self.config.pad_token_id,
+                                                                 self.config.decoder_start_token_id)
+            head.pass_hidden = True             # the call's "logits" are the head's input
+            try:
+                out = super().forward(*args, **kwargs)
+            finally:
+                del head.pass_hidden
+            out.loss = linear_cross_entropy(out.logits, head.weight, labels.to(out.logits.device))
+            out.logits = None
+            return out
+
+    # saved configurations and the Trainer know a model by its class's name
+    Model.__name__ = Model.__qualname__ = "WhisperForConditionalGeneration"
+    return Model
 
 
 def install(model, logits_in_eval: bool = True):
     """Puts the two operators into ``model``, a ``WhisperForConditionalGeneration`` (or a wrapper whose
     ``get_base_model()`` is one), in place, and returns it: the decoder's token embedding, and the loss of a call with
     ``labels``.  Such a call returns its loss and no logits (``logits`` is None); in evaluation mode it computes both
-    as before unless ``logits_in_eval`` is False.  Calls without labels, generation and saved files are untouched.
-    Weights may sit on the CPU until the first call.  Installing twice does nothing."""
+    as before unless ``logits_in_eval`` is False.  Calls without labels, generation, copies and saved files are as
+    before, and so is everything while the weights are on the CPU or in 64 bits.  Installing twice only sets
+    ``logits_in_eval``."""
     base = model.get_base_model() if hasattr(model, "get_base_model") else model
     from transformers import WhisperForConditionalGeneration
-    if not isinstance(base, WhisperForConditionalGeneration):
-        raise ValueError(f"install: {type(base).__name__} is not a WhisperForConditionalGeneration")
-    if getattr(base, "_wfe_decoder", False):
+    if isinstance(base, _model_class()):
+        base.wfe_logits_in_eval = logits_in_eval
         return model
-    from transformers.models.whisper.modeling_whisper import shift_tokens_right
+    if type(base) is not WhisperForConditionalGeneration:
+        raise ValueError(f"install: {type(base).__name__} is not a WhisperForConditionalGeneration")
     embed, head = base.get_input_embeddings(), base.get_output_embeddings()
     if type(embed) is not torch.nn.Embedding or type(head) is not torch.nn.Linear or head.bias is not None \
             or embed.max_norm is not None or embed.sparse or embed.scale_grad_by_freq:
         raise ValueError("install: the model's token embedding or output projection is not a plain one")
-    stock_forward, stock_embed, stock_head = _stock(base), _stock(embed), _stock(head)
-
-    def embed_forward(self, ids):
-        if not self.weight.is_cuda:
-            return stock_embed(self, ids)
-        return token_embedding(ids, self.weight, padding_idx=self.padding_idx)
-
-    def head_forward(self, hidden):
-        return hidden if getattr(self, "_wfe_pass_hidden", False) else stock_head(self, hidden)
-
-    @functools.wraps(type(base).forward)
-    def forward(self, *args, **kwargs):
-        labels, head = kwargs.get("labels"), self.get_output_embeddings()
-        fused = labels is not None and head.weight.is_cuda and (self.training or not logits_in_eval)
-        if not fused or kwargs.get("return_dict") is False:
-            return stock_forward(self, *args, **kwargs)
-        if labels.shape[1] > self.max_target_positions:
-            raise ValueError(f"Labels' sequence length {labels.shape[1]} cannot exceed the maximum allowed length of "
-                             f"{self.max_target_positions} tokens.")
-        kwargs["labels"] = None
-        if kwargs.get("decoder_input_ids") is None and kwargs.get("decoder_inputs_embeds") is None:
-            kwargs["decoder_input_ids"] = shift_tokens_right(labels, self.config.pad_token_id,
-                                                             self.config.decoder_start_token_id)
-        head._wfe_pass_hidden = True            # the call's "logits" are the head's input
-        try:
-            out = stock_forward(self, *args, **kwargs)
-        finally:
-            head._wfe_pass_hidden = False
-        out.loss = linear_cross_entropy(out.logits, head.weight, labels.to(out.logits.device))
-        out.logits = None
-        return out
-
-    embed.forward = types.MethodType(embed_forward, embed)
-    head.forward = types.MethodType(head_forward, head)
-    base.forward = types.MethodType(forward, base)
-    base._wfe_decoder = True
+    if any("forward" in module.__dict__ for module in (base, embed, head)):
+        raise ValueError("install: the model's forward has been replaced already (by hooks of another library, as "
+                         "device_map leaves them); install before that")
+    # subclasses, not bound functions: copies, pickles and replicas of the modules keep their own weights
+    embed.__class__, head.__class__, base.__class__ = _Embedding, _Head, _model_class()
+    base.wfe_logits_in_eval = logits_in_eval
     return model

@@ -20,8 +20,8 @@ What it does, in this process and before anything touches a GPU:
     processor whose feature extractor is the MI355X one (infer_tfs.py:27-37, evaluation.py:41-46).
 
   * with ``WFE_INSTALL_DECODER=1``, ``WhisperForConditionalGeneration.from_pretrained`` returns a model whose token
-    embedding and training loss are the HIP operators of ``wfe_amd.decoder`` (finetune.py:57-62, finetune_all.py:57-62):
-    the logits of a training step are never kept.
+    embedding and training loss are the HIP operators of ``wfe_amd.decoder``: the logits of a training step are never
+    kept.  A model that they do not fit (quantised, spread over devices) stays as it is, with a note.
 
   * for scripts that use the front end: ``WFE_DEVICE_OUTPUT`` defaults to 1 and
     ``Seq2SeqTrainingArguments`` / ``TrainingArguments`` default to ``dataloader_pin_memory=False`` (the
@@ -127,16 +127,18 @@ def _install_extractor_hook() -> None:
     WhisperProcessor.from_pretrained = classmethod(from_pretrained)
 
 
-def _install_decoder_hook() -> None:
+def _install_decoder_hook(note=sys.stderr) -> None:
     from transformers import WhisperForConditionalGeneration
     from .decoder import install
     original = WhisperForConditionalGeneration.from_pretrained.__func__
 
     def from_pretrained(cls, *args, **kwargs):
         out = original(cls, *args, **kwargs)
-        if isinstance(out, tuple):              # output_loading_info=True
-            return (install(out[0]), *out[1:])
-        return install(out)
+        try:
+            install(out[0] if isinstance(out, tuple) else out)      # (a tuple: output_loading_info=True)
+        except ValueError as e:
+            print(f"[wfe_amd.launch] decoder operators not used: {e}", file=note)
+        return out
     WhisperForConditionalGeneration.from_pretrained = classmethod(from_pretrained)
 
 
