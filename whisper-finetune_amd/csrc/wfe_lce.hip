@@ -64,13 +64,19 @@ template <> struct Elem<float> {
     p.lo = __builtin_convertvector(r - __builtin_convertvector(p.mid, f32x8), bf16x8);
     return p;
   }
-  static __device__ f32x4 mma(const Parts& a, const Parts& b, f32x4 c) {
-    c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.lo, b.hi, c, 0, 0, 0);
-    c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.hi, b.lo, c, 0, 0, 0);
-    c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.mid, b.mid, c, 0, 0, 0);
-    c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.mid, b.hi, c, 0, 0, 0);
-    c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.hi, b.mid, c, 0, 0, 0);
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.hi, b.hi, c, 0, 0, 0);
+  // the six, smallest first, each for a row of results in turn: no instruction waits for the one before it
+  template <int N>
+  static __device__ void mma(const Parts& a, const Parts (&b)[N], f32x4 (&c)[N]) {
+    const auto each = [&](auto&& term) {
+#pragma unroll
+      for (int j = 0; j < N; ++j) c[j] = term(b[j], c[j]);
+    };
+    each([&](const Parts& y, f32x4 z) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.lo, y.hi, z, 0, 0, 0); });
+    each([&](const Parts& y, f32x4 z) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.hi, y.lo, z, 0, 0, 0); });
+    each([&](const Parts& y, f32x4 z) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.mid, y.mid, z, 0, 0, 0); });
+    each([&](const Parts& y, f32x4 z) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.mid, y.hi, z, 0, 0, 0); });
+    each([&](const Parts& y, f32x4 z) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.hi, y.mid, z, 0, 0, 0); });
+    each([&](const Parts& y, f32x4 z) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.hi, y.hi, z, 0, 0, 0); });
   }
   static __device__ f32x4 mma_exact(const Frag& a, const Frag& b, f32x4 c) {
 #pragma unroll
@@ -337,9 +343,7 @@ __device__ __forceinline__ void run_tile(const TileArgs& p, int count, int id, i
         for (int j = 0; j < FB; ++j) pb[j] = Elem<T>::split(fb[j]);
 #pragma unroll
         for (int i = 0; i < FA; ++i) {
-          const auto pa = Elem<T>::split(fa[i]);
-#pragma unroll
-          for (int j = 0; j < FB; ++j) acc[i][j] = Elem<T>::mma(pa, pb[j], acc[i][j]);
+          Elem<T>::mma(Elem<T>::split(fa[i]), pb, acc[i]);
         }
       }
     };
@@ -914,7 +918,7 @@ using Small = Cfg<128, 32, 4, 1, 4, 4>;
 // the statistics of few rows: W comes from memory once, in 128-byte pieces of its rows (16 x 1280 x 51866 fp16: 29 us; 64-byte
 // pieces 35)
 using Stream = Cfg<128, 32, 4, 1, 3, 2, 2>;
-using SmallFloat = Cfg<128, 32, 4, 1, 3, 2>;
+using SmallFloat = Cfg<256, 32, 4, 1, 2, 2>;
 constexpr int kStatsRows = 128;                // fewest vocabulary rows of a tile: room for the statistics
 #ifndef WFE_PB
 #define WFE_PB 128
@@ -1077,8 +1081,11 @@ hipError_t forward(const wfe_linear_ce& d, const void* hidden, const void* weigh
   a.partial = reinterpret_cast<float2*>(ws + p.partial);
   int tiles = 0;
   if (d.rows > 0) {
-    if (sizeof(T) == 2 && d.rows <= Stream::BB) LCE_TRY((stats<T, Stream>(d, a, &tiles, stream)));
-    else LCE_TRY(with_tile<T>(d.rows, [&](auto c) { return stats<T, decltype(c)>(d, a, &tiles, stream); }));
+    bool done = false;
+    if constexpr (sizeof(T) == 2) {
+      if ((done = d.rows <= Stream::BB)) LCE_TRY((stats<T, Stream>(d, a, &tiles, stream)));
+    }
+    if (!done) LCE_TRY(with_tile<T>(d.rows, [&](auto c) { return stats<T, decltype(c)>(d, a, &tiles, stream); }));
   }
   float* row_loss = reinterpret_cast<float*>(ws + p.row_loss);
   float* total = none ? nullptr : loss;
