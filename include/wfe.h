@@ -247,7 +247,7 @@ typedef struct {
   int64_t inner;            /* rows per outer step; `rows` when there is one stride only */
   int64_t outer_stride, inner_stride, weight_stride;
   int32_t dim;              /* 1..16384 */
-  int32_t vocab;            /* 1..2^24 */
+  int32_t vocab;            /* 1..2^24; rows times vocab up to 2^37 */
   int32_t label_bits;       /* 32 or 64 */
   int32_t reduction;        /* wfe_reduction: loss has `rows` entries, or one */
   int64_t ignore_index;

@@ -26,6 +26,8 @@ def test_python_entry_points_refuse():
         emb(y, torch.empty(1, 16385))
     with pytest.raises(ValueError, match="on meta"):
         lce(h, w, y.to("meta"))
+    with pytest.raises(ValueError, match="2\\^37 logits"):
+        lce(h[:1, 0].expand(1 << 24, 8), w[:1].expand((1 << 13) + 1, 8), y[:1, 0].expand(1 << 24))
     with pytest.raises(ValueError, match="int32 or int64"):
         emb(y.bool(), w)
     for call in (lambda: lce(h, w, y), lambda: emb(y, w)):
@@ -57,7 +59,8 @@ def _emb(**kw):
 BAD_CE = [dict(dtype=3), dict(dtype=-1), dict(rows=-1), dict(rows=(1 << 24) + 1), dict(dim=0), dict(dim=16385),
           dict(vocab=0), dict(vocab=(1 << 24) + 1), dict(inner=0), dict(outer_stride=-1), dict(inner_stride=-64),
           dict(weight_stride=-1), dict(weight_stride=1 << 47), dict(label_bits=16), dict(reduction=3),
-          dict(grad_hidden_dtype=1), dict(grad_weight_dtype=1)]
+          dict(grad_hidden_dtype=1), dict(grad_weight_dtype=1),
+          dict(rows=1 << 24, vocab=(1 << 13) + 1, inner=1 << 24), dict(rows=2650000, vocab=51866, inner=2650000)]
 
 
 @pytest.mark.parametrize("bad", BAD_CE, ids=str)

@@ -137,6 +137,15 @@ def test_several_pieces_of_the_vocabulary():
     check(h, w, y, "none")
 
 
+@pytest.mark.parametrize("rows,dim,vocab,dtype,reduction", [
+    (9001, 1280, 16001, BF16, "mean"), (9000, 1273, 15999, F16, "none"), (5003, 640, 14003, F32, "sum")], ids=str)
+def test_pieces_of_a_wide_model(rows, dim, vocab, dtype, reduction):
+    """Many rows and a wide model: d in three pieces of the vocabulary, the last of them ragged."""
+    h, w, y = make(rows, dim, vocab, dtype, ignored=0.05)
+    check(h, w, y, reduction)
+    check(h, w, y, reduction, grads=(True, False))
+
+
 def test_views_strides_and_index_types():
     h, w, y = make((4, 23), 128, 1003, BF16, seed=3)
     g = torch.Generator(device="cuda").manual_seed(1)

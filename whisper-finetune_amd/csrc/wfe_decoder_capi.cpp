@@ -12,6 +12,7 @@ namespace {
 
 constexpr int64_t kMaxRows = 1 << 24, kMaxVocab = 1 << 24, kMaxDim = 16384;
 constexpr int64_t kMaxStride = (int64_t)1 << 46;
+constexpr int64_t kMaxLogits = (int64_t)1 << 37;       // a grid has fewer than 2^32 threads: 256 for 128 x 128 logits
 
 bool known_dtype(int32_t t) { return t == WFE_F32 || t == WFE_F16 || t == WFE_BF16; }
 int size_of(int32_t t) { return t == WFE_F32 ? 4 : 2; }
@@ -27,6 +28,9 @@ int check_ce(const wfe_linear_ce* d) {
     return fail(nullptr, WFE_ERR_ARG, "linear_ce: dim %d outside 1..%lld", d->dim, (long long)kMaxDim);
   if (d->vocab < 1 || d->vocab > kMaxVocab)
     return fail(nullptr, WFE_ERR_ARG, "linear_ce: vocab %d outside 1..%lld", d->vocab, (long long)kMaxVocab);
+  if (d->rows * d->vocab > kMaxLogits)
+    return fail(nullptr, WFE_ERR_ARG, "linear_ce: %lld rows by %d of the vocabulary are more than %lld logits",
+                (long long)d->rows, d->vocab, (long long)kMaxLogits);
   if (d->rows > 0 && d->inner < 1) return fail(nullptr, WFE_ERR_ARG, "linear_ce: inner %lld", (long long)d->inner);
   if (d->outer_stride < 0 || d->inner_stride < 0 || d->weight_stride < 0 || d->outer_stride > kMaxStride ||
       d->inner_stride > kMaxStride || d->weight_stride > kMaxStride)

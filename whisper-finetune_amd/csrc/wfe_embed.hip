@@ -18,9 +18,9 @@ __device__ inline long long id_at(const void* ids, int bits, int n) {
 }
 
 // 16 bytes of T.  WIDE: every row starts on 16 bytes and is whole multiples of them (the host knows); otherwise value
-// by value, with a ragged end.  The two are kernels of their own: what a wave executes for the first time comes from the L2 line by
-// line, and a gather this short is bound by that (768 rows of 1280: 16 us with both ways and a 64-bit division in one
-// kernel, see embed_kernel).
+// by value, with a ragged end.  The two are kernels of their own: what a wave executes for the first time comes from the
+// L2 line by line, and a gather this short is bound by that (768 rows of 1280: 16 us with both ways and a 64-bit division
+// in one kernel, 2.9 so).
 template <typename T, bool WIDE>
 struct Vec {
   static constexpr int kN = 16 / (int)sizeof(T);
@@ -40,26 +40,28 @@ struct Vec {
   }
 };
 
-// A wave takes TOKENS tokens' share of one slab of columns (blockIdx.y): few tokens still make many waves, many tokens
-// keep several loads of a wave in flight.
-template <typename T, bool WIDE, int TOKENS>
+// A wave takes kTokens tokens' share of one slab of columns (blockIdx.y), all their loads in flight.  Columns of 1280
+// bfloat16: 16 tokens 2.4 us, 768 2.9, 28672 (147 MB, out of the caches in part) 26; one token to a wave 3.3, 5.4 and 29.
+constexpr int kTokens = 4;
+
+template <typename T, bool WIDE>
 __global__ __launch_bounds__(256) void embed_kernel(const void* ids, int id_bits, int rows, const T* weight,
                                                     long long ld, int dim, int vocab, float scale, T* out) {
   using V = Vec<T, WIDE>;
-  const int first = __builtin_amdgcn_readfirstlane((blockIdx.x * 4 + (threadIdx.x >> 6)) * TOKENS);
+  const int first = __builtin_amdgcn_readfirstlane((blockIdx.x * 4 + (threadIdx.x >> 6)) * kTokens);
   const int d = (blockIdx.y * 64 + (threadIdx.x & 63)) * V::kN;
   if (d >= dim) return;
-  V v[TOKENS];
-  bool known[TOKENS];
+  V v[kTokens];
+  bool known[kTokens];
 #pragma unroll
-  for (int k = 0; k < TOKENS; ++k) {
+  for (int k = 0; k < kTokens; ++k) {
     const int n = first + k;
     const long long id = n < rows ? id_at(ids, id_bits, n) : -1;
     known[k] = id >= 0 && id < vocab;
     v[k].load(weight + (known[k] ? id : 0) * ld + d, dim - d);
   }
 #pragma unroll
-  for (int k = 0; k < TOKENS; ++k) {
+  for (int k = 0; k < kTokens; ++k) {
     if (first + k >= rows) break;
 #pragma unroll
     for (int e = 0; e < V::kN; ++e)
@@ -155,6 +157,7 @@ __global__ __launch_bounds__(kSortWaves * 64) void embed_sort_kernel(const void*
       const int at = place[wave][b];
       if (here && row == b) order[at + __popcll(same & ((1ull << lane) - 1))] = n;
       if (lane == 0) place[wave][b] = at + __popcll(same);
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");      // the other lanes read it the next time
       left &= ~same;
     }
   };
@@ -357,14 +360,10 @@ template <typename T, bool WIDE>
 hipError_t embed_as(const wfe_embedding_desc& d, const void* ids, const void* weight, void* out, hipStream_t stream) {
   constexpr int kSlab = 64 * (16 / (int)sizeof(T));
   const unsigned slabs = (d.dim + kSlab - 1) / kSlab;
-  auto go = [&](auto* kernel, int tokens) {
-    kernel<<<dim3((unsigned)((d.rows + 4 * tokens - 1) / (4 * tokens)), slabs), dim3(256), 0, stream>>>(
-        ids, d.id_bits, (int)d.rows, static_cast<const T*>(weight), d.weight_stride, d.dim, d.vocab, d.scale,
-        static_cast<T*>(out));
-    return hipGetLastError();
-  };
-  // 256 CUs hold about 8 of these waves each without waiting for each other's loads; beyond that a wave takes four tokens
-  return d.rows * slabs > 8 * 1024 ? go(embed_kernel<T, WIDE, 4>, 4) : go(embed_kernel<T, WIDE, 1>, 1);
+  embed_kernel<T, WIDE><<<dim3((unsigned)((d.rows + 4 * kTokens - 1) / (4 * kTokens)), slabs), dim3(256), 0, stream>>>(
+      ids, d.id_bits, (int)d.rows, static_cast<const T*>(weight), d.weight_stride, d.dim, d.vocab, d.scale,
+      static_cast<T*>(out));
+  return hipGetLastError();
 }
 
 template <typename T>

@@ -16,6 +16,8 @@
 #include <hip/hip_bf16.h>
 #include <hip/hip_fp16.h>
 
+#include <type_traits>
+
 #include "wfe_decoder.h"
 
 namespace wfe {
@@ -90,7 +92,6 @@ template <> struct Elem<float> {
 
 constexpr int kKElems = 32;                                // depth of a K tile
 template <typename T> constexpr int kKBytes = kKElems * (int)sizeof(T);
-constexpr int kPadBytes = 128;                             // packed rows are whole multiples of this
 constexpr int kPadRows = 64;                               // zeros follow the kept rows up to a multiple of this
 constexpr float kLog2e = 1.44269504088896340736f;
 
@@ -342,8 +343,15 @@ __device__ __forceinline__ void run_tile(const TileArgs& p, int count, int id, i
 #pragma unroll
         for (int j = 0; j < FB; ++j) pb[j] = Elem<T>::split(fb[j]);
 #pragma unroll
-        for (int i = 0; i < FA; ++i) {
-          Elem<T>::mma(Elem<T>::split(fa[i]), pb, acc[i]);
+        for (int i = 0; i < FA; ++i) Elem<T>::mma(Elem<T>::split(fa[i]), pb, acc[i]);
+        // The order to issue them in: the splitting that the first products wait for, then one product to three vector
+        // instructions.  Left to itself the compiler bunches them (full step in float32, 424 x 512 x 51866: z 90 us, the
+        // gradients 170; so 83 and 154).
+        __builtin_amdgcn_sched_group_barrier(0x002, 27 * (FA + FB), 0);
+#pragma unroll
+        for (int i = 0; i < 6 * FA * FB; ++i) {
+          __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+          __builtin_amdgcn_sched_group_barrier(0x002, 3, 0);
         }
       }
     };
@@ -473,8 +481,8 @@ __device__ __forceinline__ void run_tile(const TileArgs& p, int count, int id, i
       p.partial[(long long)ta * p.row_pad + b0 + b] = make_float2(top, sum);
     }
   } else if constexpr (MODE == kProb) {
-    // d rounded once to the type of the products that follow: half a step (2^-9 of itself in bfloat16), the same that
-    // rounding the gradients themselves costs
+    // d rounded once to the type of the products that follow: at most half a step (2^-8 of itself in bfloat16), the same
+    // that rounding the gradients themselves costs
     T* out = static_cast<T*>(p.prob);
 #pragma unroll
     for (int j = 0; j < FB; ++j) {
@@ -548,7 +556,8 @@ __device__ inline int tile_of(int b, int tiles) {
 }
 
 // The kept rows as strips of a tile's width; the rows that are left over, if they are few, take a narrower tile of the
-// same threads (552 rows as 2 x 256 + 64 instead of 3 x 256).
+// same threads (552 rows as 2 x 256 + 64 instead of 3 x 256: z of 552 x 768 x 51866 takes 62 us instead of 73, of 100 rows 18
+// instead of 25, of 280 float32 rows of 384 97 instead of 176).
 template <class C>
 struct Strips {
   static constexpr bool kNarrow = C::BB >= 128;
@@ -599,7 +608,7 @@ __global__ __launch_bounds__(C::kThreads, C::kWavesPerSimd) void lce_logits_kern
 
 // DHID has few tiles of its own, so its K, the vocabulary, is split.  Beside DWEI: parts of half a CU's share of all
 // the work.  Alone: the number of parts (of up to 8, or about one round) that leaves the fewest CUs idle in the last
-// round.
+// round.  (480 x 1280 x 51866 bfloat16, 10 tiles: alone 69 us, unsplit 833; beside DWEI 173, unsplit 1071.)
 struct SplitRule {
   int dim_tiles, bb, piece_steps, dwei_tiles, ke, slots, most;
 };
@@ -625,7 +634,8 @@ __device__ inline int dhid_splits(const SplitRule& r, int count) {
 }
 
 // The gradients' products over one piece, and the next piece's d, in one grid: long tiles first, so that the short
-// ones fill the CUs that run out of them.
+// ones fill the CUs that run out of them.  (4500 x 1280 x 51866 bfloat16, all but the first of four pieces' d: 1.64 TFLOP in
+// 1.56 ms, 1.06 PFLOP/s.)
 struct GradArgs {
   TileArgs t;
   SplitRule rule;
@@ -693,7 +703,8 @@ __device__ inline void copy_row(const T* in, T* out, int dim, int dim_pad, int l
 }
 
 // Block b takes rows [b per_block, ...): the kept rows before it are counted again by every block (a read of at most
-// all labels, out of L2), which saves a pass and its launch.
+// all labels, out of L2), which saves a pass and its launch.  1 row 3.4 us, 768 of 1280 bfloat16 5.2, 7168 14.6 (some 4500
+// kept, 23 MB read and written).
 constexpr int kPackRows = 4;
 
 template <typename T, bool WIDE>
@@ -751,7 +762,7 @@ __global__ __launch_bounds__(256) void lce_pack_kernel(const PackArgs p) {
   }
 }
 
-// max |g| over the kept rows
+// max |g| over the kept rows (a few hundred: 4.5 us)
 __global__ __launch_bounds__(1024) void lce_top_kernel(const float* upstream, LceState st, float* factor) {
   __shared__ float tops[16];
   const int count = st.head[0];
@@ -767,7 +778,8 @@ __global__ __launch_bounds__(1024) void lce_top_kernel(const float* upstream, Lc
 }
 
 // A loss weighted row by row (upstream of WFE_REDUCE_NONE): rows times g_n / max |g| for DWEI, rounded to their type
-// once more; within [-1, 1] times the row, so that half precision neither overflows nor loses small weights first.
+// once more; within [-1, 1] times the row, so that half precision neither overflows nor loses small weights first.  A
+// few hundred rows of 384 float32: 4.7 us.
 template <typename T>
 __global__ __launch_bounds__(256) void lce_weigh_kernel(const void* packed, void* weighted, int dim_pad, LceState st,
                                                         const float* upstream, const float* top) {
@@ -787,7 +799,7 @@ __global__ __launch_bounds__(256) void lce_weigh_kernel(const void* packed, void
   }
 }
 
-// W with rows that the tiles cannot read in place (odd sizes, strides or alignment): one padded copy
+// W with rows that the tiles cannot read in place (odd sizes, strides or alignment): one padded copy (5003 x 250: 4.2 us)
 template <typename T>
 __global__ __launch_bounds__(256) void lce_pad_weight_kernel(const T* weight, long long ld, T* out, int dim,
                                                              int dim_pad, int vocab) {
@@ -798,7 +810,8 @@ __global__ __launch_bounds__(256) void lce_pad_weight_kernel(const T* weight, lo
 
 // ---- losses out of the tiles' statistics --------------------------------------------------------------------
 // 16 rows per block and step, 64 threads per row over the vocabulary tiles.  A grid of one block takes all rows and adds
-// their losses up as well (total != null).
+// their losses up as well (total != null): up to 64 rows, 4 steps of at most 2 us, against 4.8 us of the launch that more
+// rows take for it.  4 to 5 us in all, reads one after the other rather than bytes.
 constexpr int kLossParts = 64, kLossSteps = 4;
 
 __device__ inline void merge(float& top, float& sum, float2 o) {
@@ -858,13 +871,15 @@ __global__ __launch_bounds__(1024) void lce_loss_kernel(const float2* partial, i
   if (total) sum_losses(row_loss, count, total, mean);
 }
 
-// sum or mean of the kept rows' losses, in float64 and in a fixed order.  (A launch of its own: one block telling the
-// last of the others by a counter needs every block's writes out of its XCD's L2 first, which took 50 us.)
+// sum or mean of the kept rows' losses, in float64 and in a fixed order.  (A launch of its own, 4.8 us: one block telling the
+// last of the others by a counter needs every block's writes out of its XCD's L2 first, which took 50 us with fences;
+// with every value written through 7.2 us for losses and total, as much as it saves where few rows are scored.)
 __global__ __launch_bounds__(1024) void lce_total_kernel(const float* row_loss, LceState st, float* total, int mean) {
   sum_losses(row_loss, st.head[0], total, mean);
 }
 
-// dh: the splits' sums, times g, to every row's place; zeros for ignored rows.  A wave takes 256 columns of a row.
+// dh: the splits' sums, times g, to every row's place; zeros for ignored rows.  A wave takes 256 columns of a row.  Reads what
+// the splits wrote, 8 loads in flight: 480 kept rows of 1280 11.5 us, 4500 18.5.
 struct DhidArgs {
   const float* acc;
   SplitRule rule;
@@ -912,25 +927,34 @@ __global__ __launch_bounds__(256) void lce_dhid_kernel(const DhidArgs p) {
 }
 
 // ---- host side ----------------------------------------------------------------------------------------------
+// The tiles.  What bounds the large products is the clock under the matrix instructions' power (2.0 - 2.2 GHz of 2.4): z of
+// 4096 x 1280 x 65536 bfloat16 takes 652 us (1054 TFLOP/s), the library's product of that shape 645, and zeros less than
+// either.  A step of 32 of a 256 x 256 tile takes 0.785 us on its CU and a tile 7.7 us more (the first fetches, the
+// results), so that tiles of 192, 224 or 320 columns cost more per product and won only where they saved a round of all CUs.
+// Four K tiles in LDS (128 KB): with the two groups of waves taking turns no wave waits for a fetch.
 using Large = Cfg<256, 256, 4, 2, 4, 1>;
+// float32: six products for one, and 36 vector instructions per fragment to split it, from registers that 256 x 256 results
+// would not leave.  z of 280 x 384 x 51866: 97 us.
 using Float = Cfg<128, 128, 2, 2, 2, 2>;
-using Small = Cfg<128, 32, 4, 1, 4, 4>;
-// the statistics of few rows: W comes from memory once, in 128-byte pieces of its rows (16 x 1280 x 51866 fp16: 29 us; 64-byte
-// pieces 35)
+// The statistics of few rows, a read of W.  In 2-byte types in 128-byte pieces of its rows; 1280 x 51866, 133 MB:
+// 16 rows 21 us (6.3 TB/s, part of it out of the caches), 24 with the large tile's quarter strip; 40 rows, two strips: 26 and 24.
 using Stream = Cfg<128, 32, 4, 1, 3, 2, 2>;
-using SmallFloat = Cfg<256, 32, 4, 1, 2, 2>;
-constexpr int kStatsRows = 128;                // fewest vocabulary rows of a tile: room for the statistics
-#ifndef WFE_PB
-#define WFE_PB 128
-#endif
-constexpr long long kPieceBytes = (long long)WFE_PB << 20;     // most that the d of one piece takes; two pieces are held
+// float32, 7 rows: 60 us, 69 with the tile above; 40 rows of 384: 30 either way.  (Gradients of few rows take the usual tiles:
+// 7 rows of 1280 68 us, narrow ones 71; float32 148, narrow ones 165.)
+using FloatFew = Cfg<256, 32, 4, 1, 2, 2>;
+template <typename T> using Tile = std::conditional_t<sizeof(T) == 4, Float, Large>;
+template <typename T> using FewTile = std::conditional_t<sizeof(T) == 4, FloatFew, Stream>;
 
-// calls f with the tile that suits this many rows
-template <typename T, class F>
-hipError_t with_tile(int64_t rows, F f) {
-  if constexpr (sizeof(T) == 4) return rows <= SmallFloat::BB ? f(SmallFloat{}) : f(Float{});
-  else return rows <= Small::BB ? f(Small{}) : f(Large{});
-}
+constexpr int kStatsRows = 128;                // fewest vocabulary rows of a tile: room for the statistics
+// What the d of one piece of the vocabulary takes; two are held.  Smaller ones are more launches of fewer tiles each,
+// larger ones leave the cache that a piece's two products read it from (gradients of 4500 x 1280 x 51866 bfloat16: 32 MB
+// 2.30 ms, 128 MB 1.72, 512 MB 2.06).  With many rows a piece of that size is narrow and DWEI's tiles, all rows long, are few:
+// a piece is at least so wide that the three products of a launch keep all CUs busy 1.25 times as long as one tile
+// of DWEI takes, up to kMostPieceBytes (28672 rows of 1280: 128 MB 15.5 ms, 256 to 2048 MB 10.8 to 10.3; of 384: 14.6, at 512
+// 5.1 and 1024 4.7).
+constexpr long long kPieceBytes = 128ll << 20, kMostPieceBytes = 4ll << 30;
+
+template <typename T> using Tile = std::conditional_t<sizeof(T) == 4, Float, Large>;
 
 long long up(long long x, long long to) { return (x + to - 1) / to * to; }
 
@@ -967,7 +991,13 @@ Plan make_plan(const wfe_linear_ce& d, const void* weight, bool backward, int gr
     p.row_loss = take(p.row_pad * 4);
   } else {
     const long long all = up(d.vocab, kLceRowPad);
-    long long piece = kPieceBytes / (p.row_pad * p.size) / kLceRowPad * kLceRowPad;
+    const int edge = p.size == 4 ? Float::BB : Large::BB, slots = p.size == 4 ? Float::kSlots : Large::kSlots;
+    const long long per_tile = 3 * ((p.dim_pad + edge - 1) / edge);       // tiles of a launch per `edge` of the piece
+    const long long wide = (slots * 5 / 4 + per_tile - 1) / per_tile * edge, row = p.row_pad * p.size;
+    const long long most = kMostPieceBytes / row;
+    long long piece = kPieceBytes / row;
+    if (piece < wide) piece = wide < most ? wide : most;
+    piece = piece / kLceRowPad * kLceRowPad;
     piece = piece < kLceRowPad ? kLceRowPad : piece;
     p.pieces = (int)((all + piece - 1) / piece);
     p.piece = (int)up((all + p.pieces - 1) / p.pieces, kLceRowPad);      // pieces of one size
@@ -980,8 +1010,9 @@ Plan make_plan(const wfe_linear_ce& d, const void* weight, bool backward, int gr
     p.prob[1] = p.pieces > 1 ? take(p.row_pad * p.piece * p.size) : p.prob[0];
     if (grads & WFE_GRAD_HIDDEN) {
       const long long one = p.row_pad * p.dim_pad * 4;
-      const long long most = (64ll << 20) / one;           // partial sums of dh: 64 MB, or 4 parts
-      p.splits = (int)(most < 4 ? 4 : most > 64 ? 64 : most);
+      // partial sums of dh: 64 MB; or up to 4 parts in 512 MB, behind which the tiles of one part fill the CUs twice
+      const long long most = (64ll << 20) / one, parts = (512ll << 20) / one;
+      p.splits = (int)(most > 64 ? 64 : most >= 4 ? most : parts > 4 ? 4 : parts > 1 ? parts : 1);
       p.acc = take(p.splits * one);
     }
   }
@@ -1006,7 +1037,7 @@ hipError_t launch(const A& args, long long blocks, hipStream_t stream) {
                                 (kLdsBytes<T, C>)));
     __atomic_fetch_or(&done, bit, __ATOMIC_RELAXED);
   }
-  if (blocks > 0x7ffffff0ll) return hipErrorInvalidValue;
+  if (blocks * C::kThreads > 0xffffffffll) return hipErrorInvalidValue;
   KERNEL<<<dim3((unsigned)blocks), dim3(C::kThreads), kLdsBytes<T, C>, stream>>>(args);
   return hipGetLastError();
 }
@@ -1080,13 +1111,8 @@ hipError_t forward(const wfe_linear_ce& d, const void* hidden, const void* weigh
   TileArgs a = tile_args(d, p, weight, ws, st);
   a.partial = reinterpret_cast<float2*>(ws + p.partial);
   int tiles = 0;
-  if (d.rows > 0) {
-    bool done = false;
-    if constexpr (sizeof(T) == 2) {
-      if ((done = d.rows <= Stream::BB)) LCE_TRY((stats<T, Stream>(d, a, &tiles, stream)));
-    }
-    if (!done) LCE_TRY(with_tile<T>(d.rows, [&](auto c) { return stats<T, decltype(c)>(d, a, &tiles, stream); }));
-  }
+  if (d.rows > FewTile<T>::BB) LCE_TRY((stats<T, Tile<T>>(d, a, &tiles, stream)));
+  else if (d.rows > 0) LCE_TRY((stats<T, FewTile<T>>(d, a, &tiles, stream)));
   float* row_loss = reinterpret_cast<float*>(ws + p.row_loss);
   float* total = none ? nullptr : loss;
   const bool one = d.rows <= 64;
@@ -1097,10 +1123,11 @@ hipError_t forward(const wfe_linear_ce& d, const void* hidden, const void* weigh
   return hipGetLastError();
 }
 
-template <typename T, class C>
+template <typename T>
 hipError_t gradients(const wfe_linear_ce& d, const Plan& p, GradArgs& g, char* ws, hipStream_t stream) {
+  using C = Tile<T>;
   // DWEI reads whole K tiles of rows, which PROB's narrowest strip has to have written
-  static_assert(C::KS * kKElems <= (Strips<C>::kNarrow ? Strips<C>::kQuarter : C::BB), "rows of d");
+  static_assert(C::KS * kKElems <= Strips<C>::kQuarter, "rows of d");
   const char* w = static_cast<const char*>(g.t.weight);
   g.rule.dim_tiles = tiles_of<C>(p.dim_pad, true);
   g.rule.bb = C::BB;
@@ -1165,7 +1192,7 @@ hipError_t backward(const wfe_linear_ce& d, const void* weight, const void* stat
     g.t.weighted = ws + p.weighted;
     g.t.factor = top;
   }
-  LCE_TRY(with_tile<T>(d.rows, [&](auto c) { return gradients<T, decltype(c)>(d, p, g, ws, stream); }));
+  LCE_TRY(gradients<T>(d, p, g, ws, stream));
   if (g.dhid) {
     DhidArgs k{};
     k.acc = g.t.acc;

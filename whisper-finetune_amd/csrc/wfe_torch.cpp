@@ -76,7 +76,7 @@ std::string shape_of(const Tensor& t) {
   return s + ")";
 }
 
-constexpr int64_t kMaxTokens = 1 << 24, kMaxVocab = 1 << 24, kMaxDim = 16384;
+constexpr int64_t kMaxTokens = 1 << 24, kMaxVocab = 1 << 24, kMaxDim = 16384, kMaxLogits = (int64_t)1 << 37;
 
 void check_matrix(const char* name, const Tensor& weight, const char* index_name, const Tensor& index) {
   const std::string who = std::string(name) + ": ";
@@ -111,7 +111,6 @@ void* pointer(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 
 // t with its last dimension contiguous
 Tensor dense_rows(const Tensor& t) { return t.size(-1) == 1 || t.stride(-1) == 1 ? t : t.contiguous(); }
-
 
 // Refuses to record a call on parameters that a graph of an earlier call, still alive, holds on to.  Autograd keeps one
 // accumulation node per parameter while any graph refers to it, on the stream it was made on; a captured backward pass
@@ -261,6 +260,9 @@ Tensor linear_cross_entropy(const Tensor& hidden, const Tensor& weight, const Te
   if (hidden.dim() < 1 || hidden.size(-1) != weight.size(1) || hidden.sizes().slice(0, hidden.dim() - 1) != labels.sizes())
     refuse(who + "hidden " + shape_of(hidden) + " does not fit labels " + shape_of(labels) + " and weight " +
            shape_of(weight));
+  if (labels.numel() * weight.size(0) > kMaxLogits)
+    refuse(who + std::to_string(labels.numel()) + " tokens by a vocabulary of " + std::to_string(weight.size(0)) +
+           " are more than 2^37 logits");
   if (hidden.device() != weight.device())
     refuse(who + "hidden is on " + hidden.device().str() + ", weight on " + weight.device().str());
   check_device(kCe, weight);
