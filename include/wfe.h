@@ -237,7 +237,8 @@ typedef enum { WFE_REDUCE_NONE = 0, WFE_REDUCE_SUM = 1, WFE_REDUCE_MEAN = 2 } wf
 
 /* Softmax cross entropy of labels under logits = hidden @ W^T, the logits never kept:
  *   loss_n = log sum_v exp(h_n . W_v) - h_n . W_{y_n}     (0 where y_n == ignore_index, whatever h_n holds)
- * computed with float32 logits and sums (float32 inputs: products exact to 2^-26 of themselves).  A label outside 0..vocab-1 that is not ignore_index makes the loss NaN.
+ * computed with float32 logits and sums (float32 inputs: products exact to 2^-26 of themselves).  A label outside
+ * 0..vocab-1 that is not ignore_index makes the loss NaN.
  * Hidden row n lies at hidden + (n / inner) * outer_stride + (n % inner) * inner_stride (elements), so that a
  * (batch, length, dim) view is taken as it is; rows of W at weight + v * weight_stride.  dim is contiguous. */
 typedef struct {

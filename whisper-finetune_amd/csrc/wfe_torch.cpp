@@ -1,7 +1,7 @@
 // wfe_torch.cpp -- the decoder's vocabulary operators as differentiable torch functions: a Python module
 // (wfe_amd._decoder) over the C ABI.  Host code only.  It is C++ because the calls are short: as a Python
 // torch.autograd.Function a training step of 16 x 48 tokens spent 92 us on the embedding and its gradient, of which
-// the kernels are 39 (the backward pass of a Python function runs Python on autograd's own thread).
+// the kernels are 33; from here it takes 54 (the backward pass of a Python function runs Python on autograd's own thread).
 //
 // Nothing here links to libwfe_hip.so: wfe_amd._lib loads that and hands over its entry points (bind).
 #include <ATen/autocast_mode.h>
