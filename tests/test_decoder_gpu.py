@@ -596,6 +596,26 @@ def test_embedding_strides_types_and_bad_ids():
     assert not bool(torch.autograd.grad(out, w, torch.zeros_like(out))[0].any())
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16, F32], ids=["bf16", "f16", "f32"])
+@pytest.mark.parametrize("rows", [1023, 1024, 1025, 2309])
+@pytest.mark.parametrize("dim", [7, 64, 1288])
+def test_embedding_gradient_with_bad_ids_and_strides(rows, dim, dtype):
+    """Ids out of range, padding, a common token, upstream gradients that are strided or the same for every token."""
+    d = decoder()
+    g = torch.Generator(device="cuda").manual_seed(rows + dim)
+    vocab = 1003
+    ids = tokens(rows, vocab, heavy=0.4)
+    ids[3], ids[700], ids[-1] = -1, vocab, 2 ** 40
+    padding = int(ids[0])
+    w = torch.randn(vocab, dim, generator=g, device="cuda").to(dtype).requires_grad_()
+    up = torch.randn(rows, dim + 9, generator=g, device="cuda").to(dtype)
+    for grad in (up[:, :dim].contiguous(), up[:, 8:8 + dim], up[:, 1:1 + dim], up[:1, :dim].expand(rows, dim)):
+        out = d.token_embedding(ids, w, padding_idx=padding)
+        got, = torch.autograd.grad(out, w, grad)
+        want, tol = embed_oracle(ids, grad, vocab, 1.0, padding)
+        close(got, want, tol, "dW")
+
+
 def test_embedding_gradient_leaves_masked_tokens_alone():
     """Gradients of padding tokens are dropped whatever they hold."""
     w = torch.randn(300, 64, device="cuda").requires_grad_()
