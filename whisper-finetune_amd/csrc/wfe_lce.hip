@@ -13,8 +13,6 @@
 //   DWEI   the piece's rows of dW, each written once
 // Recomputing z costs one product more than keeping (rows, vocab) logits would.
 #include <hip/hip_runtime.h>
-#include <hip/hip_bf16.h>
-#include <hip/hip_fp16.h>
 
 #include <type_traits>
 
@@ -28,7 +26,9 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
-typedef float f32x8 __attribute__((ext_vector_type(8)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 
 // Element types.  Frag: 32 K of 16 rows (or columns), a lane's share; lane group g = lane / 16 holds k = 8 g .. 8 g + 7
 // of 2-byte types, and k = 4 g .. 4 g + 3 and 16 + 4 g .. 16 + 4 g + 3 of float: any order does that is the same on both
@@ -58,13 +58,19 @@ template <> struct Elem<float> {
   struct Frag { f32x4 x[2]; };
   struct Parts { bf16x8 hi, mid, lo; };
   static __device__ Parts split(const Frag& f) {
-    const f32x8 x = __builtin_shufflevector(f.x[0], f.x[1], 0, 1, 2, 3, 4, 5, 6, 7);
-    Parts p;
-    p.hi = __builtin_convertvector(x, bf16x8);
-    const f32x8 r = x - __builtin_convertvector(p.hi, f32x8);
-    p.mid = __builtin_convertvector(r, bf16x8);
-    p.lo = __builtin_convertvector(r - __builtin_convertvector(p.mid, f32x8), bf16x8);
-    return p;
+    u32x4 hi, mid, lo;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {                // two at a time, as the conversion instruction takes them
+      const float a = f.x[k >> 1][2 * (k & 1)], b = f.x[k >> 1][2 * (k & 1) + 1];
+      hi[k] = pair(a, b);
+      const float ra = a - __builtin_bit_cast(float, hi[k] << 16), rb = b - __builtin_bit_cast(float, hi[k] & 0xffff0000u);
+      mid[k] = pair(ra, rb);
+      lo[k] = pair(ra - __builtin_bit_cast(float, mid[k] << 16), rb - __builtin_bit_cast(float, mid[k] & 0xffff0000u));
+    }
+    return {__builtin_bit_cast(bf16x8, hi), __builtin_bit_cast(bf16x8, mid), __builtin_bit_cast(bf16x8, lo)};
+  }
+  static __device__ unsigned pair(float a, float b) {
+    return __builtin_bit_cast(unsigned, __builtin_convertvector((f32x2{a, b}), bf16x2));
   }
   // the six, smallest first, each for a row of results in turn: no instruction waits for the one before it
   template <int N>
@@ -344,14 +350,14 @@ __device__ __forceinline__ void run_tile(const TileArgs& p, int count, int id, i
         for (int j = 0; j < FB; ++j) pb[j] = Elem<T>::split(fb[j]);
 #pragma unroll
         for (int i = 0; i < FA; ++i) Elem<T>::mma(Elem<T>::split(fa[i]), pb, acc[i]);
-        // The order to issue them in: the splitting that the first products wait for, then one product to three vector
-        // instructions.  Left to itself the compiler bunches them (full step in float32, 424 x 512 x 51866: z 90 us, the
-        // gradients 170; so 83 and 154).
-        __builtin_amdgcn_sched_group_barrier(0x002, 27 * (FA + FB), 0);
+        // The order to issue them in: the splitting that the first products wait for, then one product to two vector
+        // instructions.  Left to itself the compiler bunches them (201 x 384 x 51866: z 79 us, the gradients 143; so 74 and
+        // 139; 384 rows: 105 and 220, so 99 and 210).
+        __builtin_amdgcn_sched_group_barrier(0x002, 16 * (FA + FB), 0);
 #pragma unroll
         for (int i = 0; i < 6 * FA * FB; ++i) {
           __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-          __builtin_amdgcn_sched_group_barrier(0x002, 3, 0);
+          __builtin_amdgcn_sched_group_barrier(0x002, 2, 0);
         }
       }
     };
@@ -557,7 +563,7 @@ __device__ inline int tile_of(int b, int tiles) {
 
 // The kept rows as strips of a tile's width; the rows that are left over, if they are few, take a narrower tile of the
 // same threads (552 rows as 2 x 256 + 64 instead of 3 x 256: z of 552 x 768 x 51866 takes 62 us instead of 73, of 100 rows 18
-// instead of 25, of 280 float32 rows of 384 97 instead of 176).
+// instead of 25, of 280 float32 rows of 384 97 us instead of 176).
 template <class C>
 struct Strips {
   static constexpr bool kNarrow = C::BB >= 128;
@@ -933,14 +939,15 @@ __global__ __launch_bounds__(256) void lce_dhid_kernel(const DhidArgs p) {
 // results), so that tiles of 192, 224 or 320 columns cost more per product and won only where they saved a round of all CUs.
 // Four K tiles in LDS (128 KB): with the two groups of waves taking turns no wave waits for a fetch.
 using Large = Cfg<256, 256, 4, 2, 4, 1>;
-// float32: six products for one, and 36 vector instructions per fragment to split it, from registers that 256 x 256 results
-// would not leave.  z of 280 x 384 x 51866: 97 us.
+// float32: six products for one, and 44 vector instructions per fragment to split it, from registers that 256 x 256 results
+// would not leave.  z and gradients of 280 x 384 x 51866: 85 and 160 us; tiles of 128 x 256 with eight waves, one half splitting
+// while the other multiplies: 100 and 202.
 using Float = Cfg<128, 128, 2, 2, 2, 2>;
 // The statistics of few rows, a read of W.  In 2-byte types in 128-byte pieces of its rows; 1280 x 51866, 133 MB:
 // 16 rows 21 us (6.3 TB/s, part of it out of the caches), 24 with the large tile's quarter strip; 40 rows, two strips: 26 and 24.
 using Stream = Cfg<128, 32, 4, 1, 3, 2, 2>;
-// float32, 7 rows: 60 us, 69 with the tile above; 40 rows of 384: 30 either way.  (Gradients of few rows take the usual tiles:
-// 7 rows of 1280 68 us, narrow ones 71; float32 148, narrow ones 165.)
+// float32, 7 rows: 55 us, 57 with the tile above; 32 rows of 384: 20 and 21.  (Gradients of few rows take the usual tiles:
+// 7 rows of 1280 68 us, narrow ones 71; float32 142, narrow ones 165.)
 using FloatFew = Cfg<256, 32, 4, 1, 2, 2>;
 template <typename T> using Tile = std::conditional_t<sizeof(T) == 4, Float, Large>;
 template <typename T> using FewTile = std::conditional_t<sizeof(T) == 4, FloatFew, Stream>;
