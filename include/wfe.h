@@ -257,7 +257,7 @@ typedef struct {
 
 /* Bytes of the state that the forward pass leaves for the backward pass, and of the workspace of either pass (grads:
  * WFE_GRAD_ bits of the backward pass; weight: the address the pass will get, read by nobody -- rows of W that are
- * no whole multiples of 128 bytes, or not 16-byte aligned, are copied into the workspace).  Both start on 16 bytes.
+ * no whole multiples of 16 bytes, or not 16-byte aligned, are copied into the workspace).  Both start on 16 bytes.
  * Negative: a bad description. */
 int64_t wfe_linear_ce_state_bytes(const wfe_linear_ce* d);
 int64_t wfe_linear_ce_workspace_bytes(const wfe_linear_ce* d, const void* weight, int32_t backward, int32_t grads);

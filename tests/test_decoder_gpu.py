@@ -146,6 +146,30 @@ def test_pieces_of_a_wide_model(rows, dim, vocab, dtype, reduction):
     check(h, w, y, reduction, grads=(True, False))
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16, F32], ids=["bf16", "f16", "f32"])
+@pytest.mark.parametrize("rows", [9, 70, 300])
+@pytest.mark.parametrize("dim", [8, 40, 72, 104, 136, 1224])
+def test_widths_that_end_inside_a_tile(rows, dim, dtype):
+    """Rows of W are read in place up to their end: what lies between them does not matter, nor does an infinity in their
+    last values."""
+    h, w, y = make(rows, dim, 391, dtype, seed=dim, ignored=0.1)
+    base = torch.full((391, dim + 8), float("nan"), device="cuda", dtype=dtype)
+    base[:, :dim] = w
+    gaps = base[:, :dim]
+    want = check(h, w, y, "none")
+    got = check(h, gaps, y, "none")
+    assert torch.equal(want, got)
+    y[y == 17] = 18
+    h[:, -1] = 1.0
+    z = h.double() @ w.double().T
+    z[:, 17] = -float("inf")
+    gaps[17, -1] = -float("inf")
+    loss = decoder().linear_cross_entropy(h, gaps, y, reduction="none")
+    keep = y != -100
+    ref = torch.logsumexp(z, 1) - z.gather(1, y.clamp_min(0)[:, None])[:, 0]
+    assert float((loss.double() - ref)[keep].abs().max()) < 2e-5 * max(1.0, float(ref.max()))
+
+
 def test_views_strides_and_index_types():
     h, w, y = make((4, 23), 128, 1003, BF16, seed=3)
     g = torch.Generator(device="cuda").manual_seed(1)

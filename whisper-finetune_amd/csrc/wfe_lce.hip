@@ -130,25 +130,27 @@ struct Loader {
   const char* base;
   long long step;                 // bytes from one K tile to the next
   long long ld;                   // bytes
-  int k_left;                     // across: K rows that exist from the current tile on
+  int k_left;                     // K rows (across), or bytes of a row (along), that exist from the current tile on
+  const char* zeros;              // along: 16 bytes of zeros, read in place of those that do not exist
   unsigned off[kPer];
   int wave, lane;
 
   // first: row or column of the tile; limit: rows (along) or columns (across, a multiple of 16 bytes) that exist;
-  // k0 / k_rows: the first K and (across) the K rows that exist
-  __device__ void init(const T* p, long long ld_elems, int first, int limit, long long k0, long long k_rows, int w,
-                       int l) {
+  // k0: the first K; k_end: the K that exist (along: whole 16 bytes, from k0 = 0 on)
+  __device__ void init(const T* p, long long ld_elems, int first, int limit, long long k0, long long k_end, int w,
+                       int l, const T* zero = nullptr) {
     wave = w;
     lane = l;
     ld = ld_elems * (long long)sizeof(T);
     if constexpr (ACROSS) {
       base = reinterpret_cast<const char*>(p) + k0 * ld + (long long)first * sizeof(T);
       step = ld * kKElems * KS;
-      k_left = (int)(k_rows - k0);
+      k_left = (int)(k_end - k0);
     } else {
       base = reinterpret_cast<const char*>(p) + (long long)first * ld + k0 * (long long)sizeof(T);
       step = KS * kKBytes<T>;
-      k_left = 0;
+      k_left = (int)k_end * (int)sizeof(T);
+      zeros = reinterpret_cast<const char*>(zero);
     }
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
@@ -165,9 +167,10 @@ struct Loader {
       off[i] = (unsigned)(row * ld) + (unsigned)c * 16u;
     }
   }
-  // LAST: the tile may reach past the K rows that exist; those that do not are read as the last one that does (their
-  // factors on the other side are 0)
-  template <bool LAST>
+  // LAST: the tile may reach past the K that exist.  Rows that do not are read as the last one that does (their factors on
+  // the other side are 0); of a row, zeros in place of what does not (their factors are 0, but what lies there may be
+  // infinite, or nobody's memory).
+  template <bool LAST, bool TAIL>
   __device__ void issue(char* lds) {
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
@@ -177,12 +180,17 @@ struct Loader {
         const int row = (instr * 64 + lane) / kChunks;
         o -= (unsigned)(max(row - k_left + 1, 0) * ld);
       }
+      const char* from = base + o;
+      if constexpr (!ACROSS && LAST && TAIL) {
+        const int id = instr * 64 + lane, c = (id % kChunks) ^ swizzle<T, false, N, KS>(id / kChunks);
+        from = c * 16 < k_left ? from : zeros;
+      }
       __builtin_amdgcn_global_load_lds(
-          (const __attribute__((address_space(1))) void*)(base + o),
+          (const __attribute__((address_space(1))) void*)from,
           (__attribute__((address_space(3))) void*)(lds + instr * 1024), 16, 0, 0);
     }
     base += step;
-    if constexpr (ACROSS) k_left -= KS * kKElems;
+    k_left -= ACROSS ? KS * kKElems : KS * kKBytes<T>;
   }
 };
 
@@ -241,9 +249,10 @@ template <typename T, class C> constexpr int kLdsBytes = C::S * kStageBytes<T, C
 struct TileArgs {
   const void* hidden;     // packed rows (row_pad, dim_pad)
   const void* weighted;   // DWEI: the same, or rows times their own weight
-  const void* weight;     // (vocab, dim_pad) from row v0 on, weight_ld elements apart
+  const void* weight;     // (vocab, weight_cols) from row v0 on, weight_ld elements apart
   void* prob;             // d of the piece, (row_pad, prob_ld)
   long long weight_ld, prob_ld;
+  int weight_cols;        // dim, or dim_pad with zeros behind dim; 16-byte rows either way
   int dim, dim_pad, v0, piece, vocab;      // the piece holds vocabulary rows v0 .. v0 + piece - 1
   long long row_pad;
   const int* head;        // [0] kept rows
@@ -282,7 +291,7 @@ __device__ __forceinline__ void run_tile(const TileArgs& p, int count, int id, i
 
   // K range, in tiles
   int k_first = 0, k_tiles;
-  if constexpr (MODE == kStats || MODE == kProb) k_tiles = p.dim_pad / KE;
+  if constexpr (MODE == kStats || MODE == kProb) k_tiles = (p.dim + KE - 1) / KE;
   else if constexpr (MODE == kDwei) k_tiles = (count + KE - 1) / KE;
   else {
     const int all = (p.piece + KE - 1) / KE;
@@ -299,10 +308,11 @@ __device__ __forceinline__ void run_tile(const TileArgs& p, int count, int id, i
     const T* weight = static_cast<const T*>(p.weight);
     const T* prob = static_cast<const T*>(p.prob);
     if constexpr (MODE == kStats || MODE == kProb) {
-      la.init(weight, p.weight_ld, a0, p.piece, 0, 0, wave, lane);
-      lb.init(static_cast<const T*>(p.hidden), p.dim_pad, b0, b0 + BB, 0, 0, wave, lane);
+      const T* hidden = static_cast<const T*>(p.hidden);      // its first row has zeros behind dim
+      la.init(weight, p.weight_ld, a0, p.piece, 0, p.weight_cols, wave, lane, hidden + p.dim);
+      lb.init(hidden, p.dim_pad, b0, b0 + BB, 0, 0, wave, lane);
     } else if constexpr (MODE == kDhid) {
-      la.init(weight, p.weight_ld, a0, p.dim_pad, (long long)k_first * KE, p.piece, wave, lane);
+      la.init(weight, p.weight_ld, a0, p.weight_cols, (long long)k_first * KE, p.piece, wave, lane);
       lb.init(prob, p.prob_ld, b0, b0 + BB, (long long)k_first * KE, 0, wave, lane);
     } else {
       la.init(static_cast<const T*>(p.weighted), p.dim_pad, a0, p.dim_pad, 0, p.row_pad, wave, lane);
@@ -321,8 +331,8 @@ __device__ __forceinline__ void run_tile(const TileArgs& p, int count, int id, i
     constexpr int kFetches = decltype(la)::kPer + decltype(lb)::kPer;      // of every wave, per tile
     auto fetch = [&](auto last, int stage) {
       char* to = smem + stage * kStage;
-      la.template issue<decltype(last)::value>(to);
-      lb.template issue<decltype(last)::value>(to + BA * KS * kKBytes<T>);
+      la.template issue<decltype(last)::value, true>(to);
+      lb.template issue<decltype(last)::value, false>(to + BA * KS * kKBytes<T>);
     };
     typename Elem<T>::Frag fa[FA], fb[FB];
     auto read = [&](int stage, int ks) {
@@ -983,8 +993,8 @@ Plan make_plan(const wfe_linear_ce& d, const void* weight, bool backward, int gr
   p.ke = kKElems;
   p.dim_pad = lce_dim_pad(d);
   p.row_pad = lce_row_pad(d);
-  // in place: whole K tiles, 16-byte rows, offsets inside a tile in 32 bits
-  p.copy_weight = !(d.dim == p.dim_pad && (d.weight_stride * p.size) % 16 == 0 &&
+  // in place: 16-byte rows of whole 16 bytes, offsets inside a tile in 32 bits
+  p.copy_weight = !((d.dim * p.size) % 16 == 0 && (d.weight_stride * p.size) % 16 == 0 &&
                     d.weight_stride * p.size < (1ll << 22) && (reinterpret_cast<uintptr_t>(weight) & 15) == 0);
   long long at = 0;
   auto take = [&](long long bytes) {
@@ -1061,6 +1071,7 @@ TileArgs tile_args(const wfe_linear_ce& d, const Plan& p, const void* weight, ch
   a.hidden = a.weighted = st.packed;
   a.weight = p.copy_weight ? ws + p.weight : weight;
   a.weight_ld = p.copy_weight ? p.dim_pad : d.weight_stride;
+  a.weight_cols = p.copy_weight ? p.dim_pad : d.dim;
   a.dim = d.dim;
   a.dim_pad = p.dim_pad;
   a.piece = a.vocab = d.vocab;
