@@ -170,6 +170,31 @@ def test_widths_that_end_inside_a_tile(rows, dim, dtype):
     assert float((loss.double() - ref)[keep].abs().max()) < 2e-5 * max(1.0, float(ref.max()))
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16, F32], ids=["bf16", "f16", "f32"])
+@pytest.mark.parametrize("rows", [20, 300])
+def test_weights_of_rows_far_apart(rows, dtype):
+    """Upstream gradients of zero, of either sign, tiny all together and of many sizes: every row of dh is exact relative to
+    itself, dW to its largest rows."""
+    d = decoder()
+    h, w, y = make(rows, 104, 391, dtype, seed=rows, ignored=0.1)
+    g = torch.Generator(device="cuda").manual_seed(rows)
+    sign = torch.where(torch.rand(rows, generator=g, device="cuda") < 0.5, -1.0, 1.0)
+    sizes = torch.rand(rows, generator=g, device="cuda") + 0.5
+    far = sizes * 2.0 ** torch.randint(-12, 1, (rows,), generator=g, device="cuda").float()
+    some = torch.where(torch.arange(rows, device="cuda") % 3 == 0, 0.0, sizes)
+    for up in (sign * sizes * 2.0 ** -20, sign * far, some * 2.0 ** -10, some * 2.0 ** 10, torch.zeros_like(some)):
+        if dtype == F16 and float(up.abs().max()) > 100:
+            continue                                           # (its gradients leave the type's range)
+        a, b = h.clone().requires_grad_(), w.float().requires_grad_()
+        with torch.autocast("cuda", dtype=dtype, enabled=dtype != F32):
+            loss = d.linear_cross_entropy(a.float(), b, y, reduction="none")
+        ga, gb = torch.autograd.grad(loss, (a, b), up)
+        want = oracle(h, w, y, "none", up)
+        tiny = 2.0 ** -24 * float(up.abs().max()) * want[4].shape[1] if dtype == F16 else 0.0
+        close(ga.float() if dtype != F16 else ga, want[2], want[3] + HALF[dtype] * want[2].abs() + TINY[dtype], "dh")
+        close(gb, want[4], want[5] + tiny * float(h.abs().max()), "dW")
+
+
 def test_views_strides_and_index_types():
     h, w, y = make((4, 23), 128, 1003, BF16, seed=3)
     g = torch.Generator(device="cuda").manual_seed(1)

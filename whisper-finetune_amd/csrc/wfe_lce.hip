@@ -46,7 +46,7 @@ template <> struct Elem<_Float16> {
   static __device__ f32x4 mma(const Frag& a, const Frag& b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a.h, b.h, c, 0, 0, 0);
   }
-  // d is in [-1, 1]: stored times 2^14 so that small probabilities stay clear of the subnormals
+  // d is in (-2, 2), rows' own weights included: stored times 2^14 so that small probabilities stay clear of the subnormals
   static constexpr float kScale = 16384.0f;
 };
 // float32 products on the bfloat16 matrix instructions, which do 16 times the work of the float32 ones per cycle: a
@@ -102,6 +102,11 @@ constexpr int kPadRows = 64;                               // zeros follow the k
 constexpr float kLog2e = 1.44269504088896340736f;
 
 __device__ inline float exp_of(float x) { return __builtin_amdgcn_exp2f(x * kLog2e); }
+
+// A row's own weight as m 2^e, 1 <= |m| < 2 (or 0, an infinity, NaN): m goes into d before that is rounded, 2^e where it costs no
+// rounding.
+__device__ inline float weight_m(float g) { return 2.f * __builtin_amdgcn_frexp_mantf(g); }
+__device__ inline int weight_e(float g) { return __builtin_amdgcn_frexp_expf(g) - 1; }
 
 // ---- operands -------------------------------------------------------------------------------------------
 // An operand tile in LDS is either rows x 32 of K ("along": K contiguous in memory) or K rows x columns
@@ -259,6 +264,8 @@ struct TileArgs {
   const int* label;
   float* zlab;
   const float* lse;
+  const float* own;       // PROB: the rows' own weights (upstream of WFE_REDUCE_NONE, by row of hidden), or null
+  const int* index;       // rows of hidden
   float2* partial;        // STATS: (vocabulary tiles, row_pad) maximum and sum
   float* acc;             // DHID: (splits, row_pad, dim_pad)
   int first;              // DHID: acc starts with this piece
@@ -506,6 +513,7 @@ __device__ __forceinline__ void run_tile(const TileArgs& p, int count, int id, i
       const bool kept = n < count;
       const int y = kept ? p.label[n] : -1;
       const float lse = kept ? p.lse[n] : 0.f;
+      const float m = Elem<T>::kScale * (kept && p.own ? weight_m(p.own[p.index[n]]) : 1.f);
 #pragma unroll
       for (int i = 0; i < FA; ++i) {
         T d[4];
@@ -514,7 +522,7 @@ __device__ __forceinline__ void run_tile(const TileArgs& p, int count, int id, i
           const int a = a_lane + i * 16 + e, v = p.v0 + a;
           float x = exp_of(acc[i][j][e] - lse);
           x = v == y ? x - 1.f : x;
-          d[e] = static_cast<T>(kept && v < p.vocab ? x * Elem<T>::kScale : 0.f);
+          d[e] = static_cast<T>(kept && v < p.vocab ? x * m : 0.f);
         }
         __builtin_memcpy(out + (long long)n * p.prob_ld + a_lane + i * 16, d, sizeof d);
       }
@@ -778,24 +786,27 @@ __global__ __launch_bounds__(256) void lce_pack_kernel(const PackArgs p) {
   }
 }
 
-// max |g| over the kept rows (a few hundred: 4.5 us)
+// 2^e of the largest weight of the kept rows (a few hundred: 4.5 us)
 __global__ __launch_bounds__(1024) void lce_top_kernel(const float* upstream, LceState st, float* factor) {
-  __shared__ float tops[16];
+  __shared__ int tops[16];
+  constexpr int kNone = -1000;
   const int count = st.head[0];
-  float top = 0.f;
-  for (int r = threadIdx.x; r < count; r += 1024) top = fmaxf(top, fabsf(upstream[st.index[r]]));
-  for (int d = 32; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
+  int top = kNone;
+  for (int r = threadIdx.x; r < count; r += 1024) {
+    const float g = upstream[st.index[r]];
+    if (g != 0.f) top = max(top, weight_e(g));
+  }
+  for (int d = 32; d > 0; d >>= 1) top = max(top, __shfl_xor(top, d));
   if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = top;
   __syncthreads();
   if (threadIdx.x == 0) {
-    for (int i = 1; i < 16; ++i) top = fmaxf(top, tops[i]);
-    *factor = top;
+    for (int i = 1; i < 16; ++i) top = max(top, tops[i]);
+    *factor = top == kNone ? 1.f : __builtin_amdgcn_ldexpf(1.f, top);
   }
 }
 
-// A loss weighted row by row (upstream of WFE_REDUCE_NONE): rows times g_n / max |g| for DWEI, rounded to their type
-// once more; within [-1, 1] times the row, so that half precision neither overflows nor loses small weights first.  A
-// few hundred rows of 384 float32: 4.7 us.
+// A loss weighted row by row (upstream of WFE_REDUCE_NONE): rows times 2^e_n over the largest 2^e for DWEI, exact but for what
+// leaves the type's range (half precision: below 2^-24 of the largest weight's rows).  A few hundred rows of 384 float32: 4.7 us.
 template <typename T>
 __global__ __launch_bounds__(256) void lce_weigh_kernel(const void* packed, void* weighted, int dim_pad, LceState st,
                                                         const float* upstream, const float* top) {
@@ -804,13 +815,13 @@ __global__ __launch_bounds__(256) void lce_weigh_kernel(const void* packed, void
   const int r = blockIdx.x * 4 + (threadIdx.x >> 6);
   if (r >= (count + kPadRows - 1) / kPadRows * kPadRows) return;
   const bool kept = r < count;
-  float g = kept ? upstream[st.index[r]] : 0.f;
-  if (*top > 0.f) g /= *top;
+  const int e = kept ? min(weight_e(upstream[st.index[r]]) - weight_e(*top), 0) : 0;      // (a weight of 0 has any exponent)
   for (int d = (threadIdx.x & 63) * kVec; d < dim_pad; d += 64 * kVec) {
     T x[kVec];
     __builtin_memcpy(x, __builtin_assume_aligned(static_cast<const T*>(packed) + (long long)r * dim_pad + d, 16), 16);
 #pragma unroll
-    for (int e = 0; e < kVec; ++e) x[e] = kept ? static_cast<T>(static_cast<float>(x[e]) * g) : static_cast<T>(0.f);
+    for (int k = 0; k < kVec; ++k)
+      x[k] = kept ? static_cast<T>(__builtin_amdgcn_ldexpf(static_cast<float>(x[k]), e)) : static_cast<T>(0.f);
     __builtin_memcpy(__builtin_assume_aligned(static_cast<T*>(weighted) + (long long)r * dim_pad + d, 16), x, 16);
   }
 }
@@ -916,13 +927,16 @@ __global__ __launch_bounds__(256) void lce_dhid_kernel(const DhidArgs p) {
   f32x4 s = {0.f, 0.f, 0.f, 0.f};
   if (r >= 0) {
     const int splits = dhid_splits(p.rule, count);
-    float g = p.upstream[p.reduction == WFE_REDUCE_NONE ? n : 0] * (1.f / Elem<T>::kScale);
+    const bool none = p.reduction == WFE_REDUCE_NONE;
+    float g = none ? 1.f / Elem<T>::kScale : *p.upstream * (1.f / Elem<T>::kScale);
     if (p.reduction == WFE_REDUCE_MEAN) g /= (float)count;
+    const int e = none ? weight_e(p.upstream[n]) : 0;
     const float* from = p.acc + (long long)r * p.dim_pad + d;
     const long long step = p.row_pad * p.dim_pad;
 #pragma unroll 8
     for (int i = 0; i < splits; ++i) s += *reinterpret_cast<const f32x4*>(from + i * step);
-    s *= g;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s[i] = __builtin_amdgcn_ldexpf(s[i] * g, e);
   }
   const long long at = (long long)n * p.dim + d;
   const bool whole = (p.dim & 3) == 0;
@@ -1080,6 +1094,7 @@ TileArgs tile_args(const wfe_linear_ce& d, const Plan& p, const void* weight, ch
   a.label = st.label;
   a.zlab = st.zlab;
   a.lse = st.lse;
+  a.index = st.index;
   return a;
 }
 
@@ -1198,6 +1213,7 @@ hipError_t backward(const wfe_linear_ce& d, const void* weight, const void* stat
   g.t.grad_f32 = d.grad_weight_dtype == WFE_F32;
   g.t.mean = d.reduction == WFE_REDUCE_MEAN;
   g.t.factor = upstream;
+  g.t.own = d.reduction == WFE_REDUCE_NONE ? upstream : nullptr;
   g.dhid = grad_hidden && d.rows > 0;
   g.dwei = grad_weight != nullptr;
   if (g.dwei && d.reduction == WFE_REDUCE_NONE) {
