@@ -253,7 +253,7 @@ template <typename T, class C> constexpr int kLdsBytes = C::S * kStageBytes<T, C
 
 struct TileArgs {
   const void* hidden;     // packed rows (row_pad, dim_pad)
-  const void* weighted;   // DWEI: the same, or rows times their own weight
+  const void* weighted;   // DWEI: the same, or rows times 2^e of their own weight
   const void* weight;     // (vocab, weight_cols) from row v0 on, weight_ld elements apart
   void* prob;             // d of the piece, (row_pad, prob_ld)
   long long weight_ld, prob_ld;
