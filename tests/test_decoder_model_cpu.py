@@ -1,0 +1,92 @@
+"""The model path of the decoder operators (decoder.install) without a GPU: the two operators' places are taken by their
+formulas in torch, everything around them is the code that runs on one."""
+import pytest
+import torch
+import torch.nn.functional as F
+
+from wfe_amd import decoder
+
+
+@pytest.fixture
+def plain(monkeypatch):
+    """The operators as formulas, for tensors on the CPU."""
+    def loss(hidden, weight, labels, ignore_index=-100, reduction="mean"):
+        assert hidden.shape[:-1] == labels.shape and hidden.shape[-1] == weight.shape[1]
+        return F.cross_entropy((hidden @ weight.T).float().flatten(0, -2), labels.flatten(), ignore_index=ignore_index,
+                               reduction=reduction)
+
+    def embedding(ids, weight, scale=1.0, padding_idx=None):
+        return scale * F.embedding(ids, weight, padding_idx)
+    monkeypatch.setattr(decoder, "_fits", lambda weight: True)
+    monkeypatch.setattr(decoder, "linear_cross_entropy", loss)
+    monkeypatch.setattr(decoder, "token_embedding", embedding)
+
+
+def stock_model():
+    from transformers import WhisperConfig, WhisperForConditionalGeneration
+    torch.manual_seed(0)
+    cfg = WhisperConfig(vocab_size=103, num_mel_bins=8, d_model=16, encoder_layers=1, decoder_layers=1,
+                        encoder_attention_heads=2, decoder_attention_heads=2, encoder_ffn_dim=16, decoder_ffn_dim=16,
+                        max_source_positions=10, max_target_positions=8, pad_token_id=100, bos_token_id=100,
+                        eos_token_id=100, decoder_start_token_id=101, dropout=0.0, attn_implementation="eager")
+    return WhisperForConditionalGeneration(cfg).train()
+
+
+def pair():
+    """A model as it comes, and its twin with the operators."""
+    import copy
+    stock = stock_model()
+    return stock, decoder.install(copy.deepcopy(stock))
+
+
+def batch(seed=1):
+    g = torch.Generator().manual_seed(seed)
+    labels = torch.randint(0, 100, (2, 5), generator=g)
+    labels[0, 3:] = -100
+    return {"input_features": torch.randn(2, 8, 20, generator=g), "labels": labels}
+
+
+def test_output_of_a_training_call_has_a_loss_and_no_logits_in_every_form(plain):
+    stock, model = pair()
+    more = {"output_hidden_states": True, "output_attentions": True}
+    for extra in ({}, more, {"use_cache": False}):
+        want, out = stock(**batch(), **extra), model(**batch(), **extra)
+        assert type(out) is type(want)
+        assert list(out.keys()) == [k for k in want.keys() if k != "logits"]       # the loss first, as ever
+        assert "logits" not in out and out.logits is None
+        assert out[0] is out.loss and out["loss"] is out.loss and out.to_tuple()[0] is out.loss
+        assert torch.allclose(out.loss, want.loss, atol=1e-6)
+        again = type(out)(**dict(out.items()))                                     # as wrappers rebuild it from its items
+        assert again.logits is None and again.loss is out.loss
+        for k in out.keys():
+            if torch.is_tensor(out[k]):
+                assert torch.allclose(out[k], want[k], atol=1e-6), k
+        for k in ("decoder_hidden_states", "encoder_hidden_states", "decoder_attentions", "cross_attentions"):
+            assert (getattr(out, k) is None) == (getattr(want, k) is None)
+            for a, b in zip(getattr(out, k) or (), getattr(want, k) or ()):
+                assert torch.equal(a, b)
+
+
+def test_output_survives_the_conversion_of_mixed_precision_training(plain):
+    operations = pytest.importorskip("accelerate.utils.operations")
+    _, model = pair()
+    model.forward = operations.convert_outputs_to_fp32(model.forward)
+    out = model(**batch())
+    assert out.logits is None and "logits" not in out and out["loss"].dtype == torch.float32
+
+
+def test_evaluation_without_logits_predicts_nothing(plain):
+    """What the Trainer takes for predictions are the output's items apart from the loss: none of them may pass for logits."""
+    stock, model = pair()
+    decoder.install(model, logits_in_eval=False)
+    stock.eval(), model.eval()
+    with torch.no_grad():
+        want, out = stock(**batch()), model(**batch())
+    assert "logits" not in out and not any(torch.is_tensor(v) and v.shape == (2, 5, 16) for v in out.values())
+    assert torch.allclose(out.loss, want.loss, atol=1e-6)
+
+
+def test_a_call_for_tuples_is_as_before(plain):
+    stock, model = pair()
+    a, b = (m(**batch(), return_dict=False) for m in (stock, model))
+    assert isinstance(b, tuple) and len(a) == len(b) and torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])

@@ -105,7 +105,8 @@ def _model_class():
         def forward(self, *args, **kwargs):
             labels, head = kwargs.get("labels"), self.get_output_embeddings()
             fused = labels is not None and _fits(head.weight) and (self.training or not self.wfe_logits_in_eval)
-            if not fused or kwargs.get("return_dict") is False:
+            as_tuple = kwargs.get("return_dict") is False or kwargs.get("return_dict") is None and not self.config.return_dict
+            if not fused or as_tuple:
                 return super().forward(*args, **kwargs)
             if labels.shape[1] > self.max_target_positions:
                 raise ValueError(f"labels of {labels.shape[1]} tokens are longer than max_target_positions "
@@ -119,9 +120,9 @@ def _model_class():
                 out = super().forward(*args, **kwargs)
             finally:
                 del head.pass_hidden
-            out.loss = linear_cross_entropy(out.logits, head.weight, labels.to(out.logits.device))
-            out.logits = None
-            return out
+            loss = linear_cross_entropy(out.logits, head.weight, labels.to(out.logits.device))
+            # an output of its own: the entries of a mapping stay what they were made as, whatever its attributes are set to
+            return type(out)(loss=loss, logits=None, **{k: v for k, v in out.items() if k not in ("loss", "logits")})
 
     # saved configurations and the Trainer know a model by its class's name
     Model.__name__ = Model.__qualname__ = "WhisperForConditionalGeneration"
