@@ -3,6 +3,7 @@ formulas in torch, everything around them is the code that runs on one."""
 import pytest
 import torch
 import torch.nn.functional as F
+import torch.nn.utils.parametrize
 
 from wfe_amd import decoder
 
@@ -90,3 +91,72 @@ def test_a_call_for_tuples_is_as_before(plain):
     stock, model = pair()
     a, b = (m(**batch(), return_dict=False) for m in (stock, model))
     assert isinstance(b, tuple) and len(a) == len(b) and torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+class Wrapped(torch.nn.Module):
+    """An output projection with an adapter around it."""
+
+    def __init__(self, inner):
+        super().__init__()
+        self.inner, self.more = inner, torch.nn.Linear(inner.in_features, inner.out_features, bias=False)
+
+    @property
+    def weight(self):
+        return self.inner.weight
+
+    def forward(self, x):
+        return self.inner(x) + self.more(x)
+
+
+def other_head(model, how):
+    head = model.get_output_embeddings()
+    torch.manual_seed(3)
+    if how == "resized":
+        model.resize_token_embeddings(110)
+    elif how == "bias":
+        model.set_output_embeddings(torch.nn.Linear(16, 103))
+    elif how == "bias on the same":
+        head.bias = torch.nn.Parameter(torch.randn(103))
+    elif how == "adapter":
+        model.set_output_embeddings(Wrapped(head))
+    elif how == "forward replaced":
+        head.forward = lambda x: torch.nn.functional.linear(x, 2 * head.weight)
+    elif how == "hook":
+        head.register_forward_hook(lambda module, args, out: 2 * out)
+    elif how == "pre-hook":
+        head.register_forward_pre_hook(lambda module, args: (2 * args[0],))
+    elif how == "parametrized":
+        class Doubled(torch.nn.Module):
+            def forward(self, w):
+                return 2 * w
+        torch.nn.utils.parametrize.register_parametrization(head, "weight", Doubled())
+
+
+@pytest.mark.parametrize("how", ["resized", "bias", "bias on the same", "adapter", "forward replaced", "hook", "pre-hook",
+                                 "parametrized"])
+def test_an_output_projection_changed_after_install_counts(plain, how):
+    """What install found may be replaced, wrapped or hooked later on; the loss is that of the projection as it then is."""
+    stock, model = pair()
+    for m in (stock, model):
+        other_head(m, how)
+    want, out = stock(**batch()), model(**batch())
+    assert torch.allclose(out.loss, want.loss, atol=1e-5), (out.loss.detach(), want.loss.detach())
+    for o in (want, out):
+        o.loss.backward()
+    for (name, p), q in zip(stock.named_parameters(), model.parameters()):
+        assert (p.grad is None) == (q.grad is None), name
+        assert p.grad is None or torch.allclose(p.grad, q.grad, atol=1e-5), name
+
+
+def test_weights_that_are_no_plain_matrix():
+    """A matrix that another library holds in pieces, or as a tensor type of its own, is only that library's to read."""
+    class Fake:
+        is_cuda, dtype, shape = True, torch.float32, (4, 4)
+
+        def dim(self):
+            return 2
+
+    class Own(torch.nn.Parameter):
+        is_cuda = True
+    assert not decoder._fits(torch.nn.Parameter(torch.zeros(4, 4)))               # on the CPU
+    assert not decoder._fits(Fake()) and not decoder._fits(Own(torch.zeros(4, 4)))

@@ -76,7 +76,15 @@ _TYPES = (torch.float32, torch.float16, torch.bfloat16)
 
 
 def _fits(weight: torch.Tensor) -> bool:
-    return weight.is_cuda and weight.dtype in _TYPES
+    # (libraries that shard or quantise hold weights as flat pieces or as tensor types of their own)
+    return type(weight) in (torch.Tensor, torch.nn.Parameter) and weight.dim() == 2 and weight.is_cuda \
+        and weight.dtype in _TYPES
+
+
+def _plain(module, kind) -> bool:
+    """Whether ``module`` computes what a ``kind`` (a class of this file) does and nothing beside it."""
+    return type(module) is kind and "forward" not in module.__dict__ and not (
+        module._forward_hooks or module._forward_pre_hooks or module._backward_hooks or module._backward_pre_hooks)
 
 
 class _Embedding(torch.nn.Embedding):
@@ -104,7 +112,9 @@ def _model_class():
         @functools.wraps(WhisperForConditionalGeneration.forward)
         def forward(self, *args, **kwargs):
             labels, head = kwargs.get("labels"), self.get_output_embeddings()
-            fused = labels is not None and _fits(head.weight) and (self.training or not self.wfe_logits_in_eval)
+            # the projection may have been replaced, wrapped or hooked since install: then it is called as it is
+            fused = labels is not None and (self.training or not self.wfe_logits_in_eval) \
+                and _plain(head, _Head) and head.bias is None and _fits(head.weight)
             as_tuple = kwargs.get("return_dict") is False or kwargs.get("return_dict") is None and not self.config.return_dict
             if not fused or as_tuple:
                 return super().forward(*args, **kwargs)
