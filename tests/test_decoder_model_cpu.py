@@ -160,3 +160,62 @@ def test_weights_that_are_no_plain_matrix():
         is_cuda = True
     assert not decoder._fits(torch.nn.Parameter(torch.zeros(4, 4)))               # on the CPU
     assert not decoder._fits(Fake()) and not decoder._fits(Own(torch.zeros(4, 4)))
+
+
+def test_two_threads_on_one_model(plain):
+    """A training call waits in the middle of the decoder while another thread asks the same model for logits, or trains."""
+    import threading
+    for second in ("logits", "loss"):
+        stock, model = pair()
+        inputs, other = batch(), batch(2)
+        if second == "logits":
+            other = {"input_features": other["input_features"], "decoder_input_ids": torch.tensor([[101, 1, 2], [101, 3, 4]])}
+        inside, go_on = threading.Event(), threading.Event()
+        first = []
+
+        def wait(module, args, output):
+            if threading.current_thread() is first[0]:
+                inside.set()
+                assert go_on.wait(60)
+        model.model.decoder.register_forward_hook(wait)
+        got, errors = {}, []
+
+        def train():
+            try:
+                got["first"] = model(**inputs)
+            except Exception as e:  # noqa: BLE001 -- reported below
+                errors.append(e)
+        first.append(threading.Thread(target=train))
+        first[0].start()
+        try:
+            assert inside.wait(60)
+            got["second"] = model(**other)
+        finally:
+            go_on.set()
+            first[0].join()
+        assert not errors, errors
+        assert torch.allclose(got["first"].loss, stock(**inputs).loss, atol=1e-6)
+        want = stock(**other)
+        if second == "logits":
+            assert torch.equal(got["second"].logits, want.logits)
+        else:
+            assert torch.allclose(got["second"].loss, want.loss, atol=1e-6)
+
+
+def test_arguments_by_position(plain):
+    """Every argument of a call may come by position, labels among them."""
+    import inspect
+    stock, model = pair()
+    names = list(inspect.signature(stock.forward).parameters)
+    given = batch()
+    by_position = [given.get(name) for name in names[:names.index("labels") + 1]]
+    want, out = stock(**given), model(*by_position)
+    assert torch.allclose(out.loss, want.loss, atol=1e-6) and "logits" not in out
+    out = model(given["input_features"], labels=given["labels"], num_items_in_batch=7)     # as a Trainer calls it
+    assert torch.allclose(out.loss, want.loss, atol=1e-6) and "logits" not in out
+    seen = {}
+    model.model.register_forward_pre_hook(lambda module, args, kwargs: seen.update(kwargs), with_kwargs=True)
+    model(**given, num_items_in_batch=7, use_cache=False)
+    assert set(seen) == {"input_features", "decoder_input_ids", "num_items_in_batch", "use_cache", "return_dict"}
+    with pytest.raises(TypeError):
+        model(given["input_features"], input_features=given["input_features"], labels=given["labels"])

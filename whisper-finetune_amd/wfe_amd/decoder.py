@@ -16,6 +16,7 @@ from __future__ import annotations
 
 import ctypes as C
 import functools
+import inspect
 import os
 from typing import Optional
 
@@ -82,7 +83,7 @@ def _fits(weight: torch.Tensor) -> bool:
 
 
 def _plain(module, kind) -> bool:
-    """Whether ``module`` computes what a ``kind`` (a class of this file) does and nothing beside it."""
+    """Whether ``module`` computes what a ``kind`` does and nothing beside it."""
     return type(module) is kind and "forward" not in module.__dict__ and not (
         module._forward_hooks or module._forward_pre_hooks or module._backward_hooks or module._backward_pre_hooks)
 
@@ -94,45 +95,43 @@ class _Embedding(torch.nn.Embedding):
         return token_embedding(ids, self.weight, padding_idx=self.padding_idx)
 
 
-class _Head(torch.nn.Linear):
-    pass_hidden = False                         # a call wants the head's input instead of the logits
-
-    def forward(self, hidden):
-        return hidden if self.pass_hidden else super().forward(hidden)
-
-
 @functools.lru_cache(maxsize=None)
 def _model_class():
     from transformers import WhisperForConditionalGeneration
+    from transformers.modeling_outputs import Seq2SeqLMOutput
     from transformers.models.whisper.modeling_whisper import shift_tokens_right
+    signature = inspect.signature(WhisperForConditionalGeneration.forward)
+    more = next((p.name for p in signature.parameters.values() if p.kind is p.VAR_KEYWORD), None)
 
     class Model(WhisperForConditionalGeneration):
         wfe_logits_in_eval = True
 
         @functools.wraps(WhisperForConditionalGeneration.forward)
         def forward(self, *args, **kwargs):
-            labels, head = kwargs.get("labels"), self.get_output_embeddings()
-            # the projection may have been replaced, wrapped or hooked since install: then it is called as it is
-            fused = labels is not None and (self.training or not self.wfe_logits_in_eval) \
-                and _plain(head, _Head) and head.bias is None and _fits(head.weight)
-            as_tuple = kwargs.get("return_dict") is False or kwargs.get("return_dict") is None and not self.config.return_dict
-            if not fused or as_tuple:
-                return super().forward(*args, **kwargs)
+            if self.training or not self.wfe_logits_in_eval:
+                given = dict(signature.bind(self, *args, **kwargs).arguments)
+                given.update(given.pop(more, {}))
+                labels, return_dict, head = given.get("labels"), given.get("return_dict"), self.get_output_embeddings()
+                as_tuple = not (self.config.return_dict if return_dict is None else return_dict)
+                # the projection may have been replaced, wrapped or hooked since install: then it is called as it is
+                if labels is not None and not as_tuple and _plain(head, torch.nn.Linear) and head.bias is None \
+                        and _fits(head.weight):
+                    del given["self"], given["labels"]
+                    return self._wfe_loss(head.weight, labels, {**given, "return_dict": True})
+            return super().forward(*args, **kwargs)
+
+        def _wfe_loss(self, weight, labels, given):
+            """The call with labels: the decoder's last hidden states into the loss, the projection itself not called."""
             if labels.shape[1] > self.max_target_positions:
                 raise ValueError(f"labels of {labels.shape[1]} tokens are longer than max_target_positions "
                                  f"({self.max_target_positions})")
-            kwargs["labels"] = None
-            if kwargs.get("decoder_input_ids") is None and kwargs.get("decoder_inputs_embeds") is None:
-                kwargs["decoder_input_ids"] = shift_tokens_right(labels, self.config.pad_token_id,
-                                                                 self.config.decoder_start_token_id)
-            head.pass_hidden = True             # the call's "logits" are the head's input
-            try:
-                out = super().forward(*args, **kwargs)
-            finally:
-                del head.pass_hidden
-            loss = linear_cross_entropy(out.logits, head.weight, labels.to(out.logits.device))
-            # an output of its own: the entries of a mapping stay what they were made as, whatever its attributes are set to
-            return type(out)(loss=loss, logits=None, **{k: v for k, v in out.items() if k not in ("loss", "logits")})
+            if given.get("decoder_input_ids") is None and given.get("decoder_inputs_embeds") is None:
+                given["decoder_input_ids"] = shift_tokens_right(labels, self.config.pad_token_id,
+                                                                self.config.decoder_start_token_id)
+            out = self.model(**given)
+            hidden = out.last_hidden_state
+            loss = linear_cross_entropy(hidden, weight, labels.to(hidden.device))
+            return Seq2SeqLMOutput(loss=loss, **{k: v for k, v in out.items() if k != "last_hidden_state"})
 
     # saved configurations and the Trainer know a model by its class's name
     Model.__name__ = Model.__qualname__ = "WhisperForConditionalGeneration"
@@ -161,6 +160,6 @@ def install(model, logits_in_eval: bool = True):
         raise ValueError("install: the model's forward has been replaced already (by hooks of another library, as "
                          "device_map leaves them); install before that")
     # subclasses, not bound functions: copies, pickles and replicas of the modules keep their own weights
-    embed.__class__, head.__class__, base.__class__ = _Embedding, _Head, _model_class()
+    embed.__class__, base.__class__ = _Embedding, _model_class()
     base.wfe_logits_in_eval = logits_in_eval
     return model
