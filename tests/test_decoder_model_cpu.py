@@ -219,3 +219,38 @@ def test_arguments_by_position(plain):
     assert set(seen) == {"input_features", "decoder_input_ids", "num_items_in_batch", "use_cache", "return_dict"}
     with pytest.raises(TypeError):
         model(given["input_features"], input_features=given["input_features"], labels=given["labels"])
+
+
+def test_installed_models_pickle_and_save_whole(plain, tmp_path):
+    import copy
+    import io
+    import pickle
+    stock, model = pair()
+    decoder.install(model, logits_in_eval=False)
+    want = model(**batch())
+    buffer = io.BytesIO()
+    torch.save(model, buffer)
+    buffer.seek(0)
+    for twin in (pickle.loads(pickle.dumps(model)), torch.load(buffer, weights_only=False), copy.deepcopy(model)):
+        assert type(twin) is type(model) and twin.wfe_logits_in_eval is False
+        out = twin(**batch())
+        assert torch.equal(out.loss, want.loss) and "logits" not in out
+    # in a process that has not installed anything
+    path = tmp_path / "model.pkl"
+    path.write_bytes(pickle.dumps(model.cpu()))
+    import os
+    import subprocess
+    import sys
+    package = os.path.dirname(os.path.dirname(decoder.__file__))
+    code = ("import pickle, sys; m = pickle.load(open(sys.argv[1], 'rb')); from wfe_amd import decoder; "
+            "assert type(m) is decoder._model_class() and m.wfe_logits_in_eval is False; print(type(m).__name__)")
+    done = subprocess.run([sys.executable, "-c", code, str(path)], env={**os.environ, "PYTHONPATH": package},
+                          capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0 and done.stdout.strip() == "WhisperForConditionalGeneration", done.stderr
+    model.save_pretrained(tmp_path / "saved")
+    from transformers import WhisperForConditionalGeneration
+    again = WhisperForConditionalGeneration.from_pretrained(tmp_path / "saved").train()
+    assert type(again) is WhisperForConditionalGeneration
+    assert torch.allclose(again(**batch()).loss, want.loss, atol=1e-6)
+    with pytest.raises(AttributeError):
+        decoder.no_such_name

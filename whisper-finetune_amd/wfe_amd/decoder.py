@@ -133,9 +133,15 @@ def _model_class():
             loss = linear_cross_entropy(hidden, weight, labels.to(hidden.device))
             return Seq2SeqLMOutput(loss=loss, **{k: v for k, v in out.items() if k != "last_hidden_state"})
 
-    # saved configurations and the Trainer know a model by its class's name
+    # saved configurations and the Trainer know a model by its class's name; pickles find it here by that (__getattr__)
     Model.__name__ = Model.__qualname__ = "WhisperForConditionalGeneration"
     return Model
+
+
+def __getattr__(name):
+    if name == "WhisperForConditionalGeneration":
+        return _model_class()
+    raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
 
 
 def install(model, logits_in_eval: bool = True):
