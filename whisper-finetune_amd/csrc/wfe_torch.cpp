@@ -6,6 +6,7 @@
 // Nothing here links to libwfe_hip.so: wfe_amd._lib loads that and hands over its entry points (bind).
 #include <ATen/autocast_mode.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
+#include <c10/core/AutogradState.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/extension.h>
@@ -92,6 +93,30 @@ void check_matrix(const char* name, const Tensor& weight, const char* index_name
     refuse(who + std::to_string(index.numel()) + " tokens are more than " + std::to_string(kMaxTokens));
   if (index.device() != weight.device())
     refuse(who + index_name + " are on " + index.device().str() + ", weight on " + weight.device().str());
+}
+
+// What differentiates or batches a call behind autograd's back would get the values alone: forward-mode tangents, which are
+// not tied to requires_grad, and the function transforms' wrappers.  -> its name, or null
+const char* unknown_mode(const Tensor& t) {
+  constexpr c10::DispatchKeySet wrapped({c10::DispatchKey::FuncTorchGradWrapper, c10::DispatchKey::FuncTorchBatched});
+  if (t.key_set().has_any(wrapped)) return "a function transform (torch.func)";
+  if (c10::AutogradState::get_tls_state().get_fw_grad_mode() && t.unsafeGetTensorImpl()->_fw_grad(0, t).defined())
+    return "forward-mode differentiation";
+  return nullptr;
+}
+
+void check_modes(const char* name, std::initializer_list<Tensor> inputs) {
+  for (const Tensor& t : inputs)
+    if (const char* mode = unknown_mode(t)) {
+      PyErr_SetString(PyExc_NotImplementedError, (std::string(name) + ": " + mode + " is not supported").c_str());
+      throw pybind11::error_already_set();
+    }
+}
+
+// The same in a backward pass, which runs on autograd's own threads
+void check_upstream(const char* name, const Tensor& grad) {
+  if (const char* mode = unknown_mode(grad))
+    throw std::runtime_error(std::string(name) + ": " + mode + " of the gradient is not supported");
 }
 
 void check_device(const char* name, const Tensor& weight) {
@@ -227,6 +252,7 @@ struct LinearCrossEntropy : torch::autograd::Function<LinearCrossEntropy> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     variable_list result(6);
     if (!grads[0].defined()) return result;
+    check_upstream(kCe, grads[0]);
     {
       const at::AutoDispatchBelowADInplaceOrView below;
       const auto saved = ctx->get_saved_variables();
@@ -255,6 +281,7 @@ struct LinearCrossEntropy : torch::autograd::Function<LinearCrossEntropy> {
 
 Tensor linear_cross_entropy(const Tensor& hidden, const Tensor& weight, const Tensor& labels, int64_t ignore_index,
                             int64_t reduction) {
+  check_modes(kCe, {hidden, weight, labels});
   check_matrix(kCe, weight, "labels", labels);
   const std::string who = std::string(kCe) + ": ";
   if (hidden.dim() < 1 || hidden.size(-1) != weight.size(1) || hidden.sizes().slice(0, hidden.dim() - 1) != labels.sizes())
@@ -324,6 +351,7 @@ struct TokenEmbedding : torch::autograd::Function<TokenEmbedding> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     variable_list result(4);
     if (!grads[0].defined()) return result;
+    check_upstream(kEmbed, grads[0]);
     {
       const at::AutoDispatchBelowADInplaceOrView below;
       const Tensor ids = ctx->get_saved_variables()[0];
@@ -343,6 +371,7 @@ struct TokenEmbedding : torch::autograd::Function<TokenEmbedding> {
 };
 
 Tensor token_embedding(const Tensor& ids, const Tensor& weight, double scale, std::optional<int64_t> padding_idx) {
+  check_modes(kEmbed, {ids, weight});
   check_matrix(kEmbed, weight, "ids", ids);
   int64_t padding = -1;
   if (padding_idx) {

@@ -55,7 +55,7 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, labels: tor
     ``torch.autocast`` both are cast to its type, as ``F.linear`` casts them, and gradients come in the inputs' own
     types.  Tokens whose label is ``ignore_index`` cost nothing and contribute nothing, whatever ``hidden`` holds there.
     A label outside the vocabulary makes the loss (and the gradients) NaN.  Differentiable once, in ``hidden`` and
-    ``weight``.  At most 2^24 tokens, a vocabulary of 2^24, a dim of 16384 and 2^37 logits."""
+    ``weight``, in reverse mode (forward-mode tangents and ``torch.func`` transforms raise).  At most 2^24 tokens, a vocabulary of 2^24, a dim of 16384 and 2^37 logits."""
     code = _REDUCTIONS.get(reduction)
     if code is None:
         raise ValueError(f"linear_cross_entropy: reduction {reduction!r} is not 'none', 'sum' or 'mean'")
@@ -68,7 +68,8 @@ def token_embedding(ids: torch.Tensor, weight: torch.Tensor, *, scale: float = 1
 
     ``ids`` (...) int32 or int64, ``weight`` (vocab, dim) float32, float16 or bfloat16.  The gradient of ``weight`` is
     summed in float32 over a token's occurrences in their order, the same bits every time; ``padding_idx`` (negative:
-    from the end) gets none.  An id outside the vocabulary gives a row of NaN and no gradient.  Differentiable once."""
+    from the end) gets none.  An id outside the vocabulary gives a row of NaN and no gradient.  Differentiable once, in
+    reverse mode, as above."""
     return (_module or _ext()).token_embedding(ids, weight, scale, padding_idx)
 
 
