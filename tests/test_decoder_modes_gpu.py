@@ -27,3 +27,59 @@ def test_tangents_are_refused_in_both_directions():
                 torch.autograd.grad(out, of, up, retain_graph=True)
             assert torch.autograd.grad(out, of, torch.ones_like(out))[0].shape == of.shape
         assert d.linear_cross_entropy(h, w, y).dim() == 0          # no tangent, no refusal
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32], ids=["bf16", "f16", "f32"])
+def test_saved_tensors_moved_by_hooks(dtype):
+    """What a call saves may come back as another tensor (offloading hooks bring back contiguous copies), whatever strides it
+    had: the gradients are the same bits."""
+    from wfe_amd import decoder as d
+    g = torch.Generator(device="cuda").manual_seed(1)
+    base = torch.randn(300, 200, generator=g, device="cuda").to(dtype)
+    y = torch.randint(0, 100, (40,), generator=g, device="cuda")
+    h = torch.randn(40, 64, generator=g, device="cuda").to(dtype).requires_grad_()
+    views = {"wide rows": lambda: base[:, :64], "off its alignment": lambda: base[:, 3:67], "every third": lambda: base[::3, 8:72],
+             "one row": lambda: base[:1, :64].expand(120, 64), "columns": lambda: base[:64, :150].T, "dense": lambda: base[:, :64].clone()}
+
+    def moved(t):
+        return t.detach().cpu()
+
+    def back(t):
+        return t.to("cuda")
+
+    def spread(t):
+        """Comes back with other strides than it was saved with."""
+        room = torch.full((*t.shape[:-1], t.shape[-1] + 8), 7, dtype=t.dtype, device=t.device)
+        room[..., :t.shape[-1]] = t.detach()
+        return room[..., :t.shape[-1]]
+    for name, view in views.items():
+        w = view().detach().requires_grad_()
+
+        def step():
+            out = d.token_embedding(y, w, scale=0.5)
+            loss = d.linear_cross_entropy(h + out, w, y)
+            return torch.autograd.grad(loss, (h, w))
+        want = step()
+        with torch.autograd.graph.save_on_cpu():
+            offloaded = step()
+        with torch.autograd.graph.saved_tensors_hooks(moved, back):
+            again = step()
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t, spread):
+            strided = step()
+        for other in (offloaded, again, strided):
+            for a, b in zip(want, other):
+                assert torch.equal(a, b), name
+
+
+def test_saved_tensors_changed_by_hooks_are_refused():
+    """Hooks that bring back less than was saved, or another type of it, get an error and no kernel."""
+    from wfe_amd import decoder as d
+    h, w, y = case()
+    h, w = h.requires_grad_(), w.requires_grad_()
+    for call in (lambda: d.linear_cross_entropy(h, w, y), lambda: d.token_embedding(y, w).sum()):
+        for change in (lambda t: t[:-1] if t.dim() else t, lambda t: t.to(torch.float16), lambda t: t.cpu(),
+                       lambda t: t.reshape(-1)[:0]):
+            with torch.autograd.graph.saved_tensors_hooks(lambda t: t, change):
+                out = call()
+            with pytest.raises((RuntimeError, ValueError), match="saved"):
+                torch.autograd.grad(out, w)

@@ -56,6 +56,7 @@ int dtype_code(at::ScalarType t) {
     default: return -1;
   }
 }
+at::ScalarType type_of(int32_t code) { return code == WFE_F32 ? at::kFloat : code == WFE_F16 ? at::kHalf : at::kBFloat16; }
 std::string name_of(at::ScalarType t) {        // as Python has it
   switch (t) {
     case at::kDouble: return "float64";
@@ -136,6 +137,13 @@ void* pointer(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 
 // t with its last dimension contiguous
 Tensor dense_rows(const Tensor& t) { return t.size(-1) == 1 || t.stride(-1) == 1 ? t : t.contiguous(); }
+
+// A saved tensor as it was when it was saved, strides apart: hooks on saved tensors may bring back another one.
+void check_saved(const char* name, const Tensor& t, at::IntArrayRef sizes, at::ScalarType type, const c10::Device& device) {
+  if (!t.defined() || t.layout() != at::kStrided || t.sizes() != sizes || t.scalar_type() != type || t.device() != device)
+    throw std::runtime_error(std::string(name) + ": a tensor saved for the backward pass came back with another shape, type "
+                             "or device (from hooks on saved tensors)");
+}
 
 // Refuses to record a call on parameters that a graph of an earlier call, still alive, holds on to.  Autograd keeps one
 // accumulation node per parameter while any graph refers to it, on the stream it was made on; a captured backward pass
@@ -256,9 +264,12 @@ struct LinearCrossEntropy : torch::autograd::Function<LinearCrossEntropy> {
     {
       const at::AutoDispatchBelowADInplaceOrView below;
       const auto saved = ctx->get_saved_variables();
-      const Tensor &weight = saved[0], &state = saved[1];
-      const auto d = unpacked<wfe_linear_ce>(ctx->saved_data["desc"].toStringRef());
+      auto d = unpacked<wfe_linear_ce>(ctx->saved_data["desc"].toStringRef());
       const auto types = ctx->saved_data["types"].toIntVector();
+      check_saved(kCe, saved[0], {d.vocab, d.dim}, type_of(d.dtype), grads[0].device());
+      check_saved(kCe, saved[1], {entry.ce_state(&d)}, at::kByte, grads[0].device());
+      const Tensor weight = dense_rows(saved[0]), state = saved[1].contiguous();
+      d.weight_stride = weight.stride(0);
       const Tensor upstream = grads[0].to(at::kFloat).contiguous();
       Tensor grad_hidden, grad_weight;
       const auto kind = [&](int32_t code) { return code == WFE_F32 ? at::kFloat : weight.scalar_type(); };
@@ -354,8 +365,11 @@ struct TokenEmbedding : torch::autograd::Function<TokenEmbedding> {
     check_upstream(kEmbed, grads[0]);
     {
       const at::AutoDispatchBelowADInplaceOrView below;
-      const Tensor ids = ctx->get_saved_variables()[0];
+      const Tensor saved = ctx->get_saved_variables()[0];
       auto d = unpacked<wfe_embedding_desc>(ctx->saved_data["desc"].toStringRef());
+      check_saved(kEmbed, saved, grads[0].sizes().slice(0, grads[0].dim() - 1), d.id_bits == 64 ? at::kLong : at::kInt,
+                  grads[0].device());
+      const Tensor ids = saved.contiguous();
       Tensor rows = dense_rows(grads[0]);
       if (!rows.is_contiguous()) rows = rows.reshape({-1, d.dim});     // a view where the leading dimensions allow one
       d.grad_stride = rows.is_contiguous() ? d.dim : rows.stride(0);
