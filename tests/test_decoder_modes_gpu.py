@@ -83,3 +83,31 @@ def test_saved_tensors_changed_by_hooks_are_refused():
                 out = call()
             with pytest.raises((RuntimeError, ValueError), match="saved"):
                 torch.autograd.grad(out, w)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32], ids=["bf16", "f16", "f32"])
+def test_lazily_negated_views(dtype):
+    """torch keeps the sign of some views (the imaginary part of a conjugate) apart from their memory."""
+    from wfe_amd import decoder as d
+    h, w, y = case()
+    h, w = h.to(dtype), w.to(dtype)
+    up = torch.linspace(-1, 1, 6, device="cuda")
+
+    def step(h, w, y, up):
+        h, w = h.detach().requires_grad_(), w.detach().requires_grad_()
+        loss = d.linear_cross_entropy(h, w, y, reduction="none")
+        out = d.token_embedding(y, w)
+        with torch.no_grad():
+            plain = d.linear_cross_entropy(h, w, y), d.token_embedding(y, w)
+        return (loss, out, *plain, *torch.autograd.grad(loss, (h, w), up),
+                *torch.autograd.grad(out, w, up[:, None].to(dtype).expand_as(out)))
+    want = step(h, w, y, up)
+    neg = torch._neg_view
+    for given in ((neg(-h), w, y, up), (h, neg(-w), y, up), (h, w, neg(-y), up), (h, w, y, neg(-up)),
+                  (neg(-h.expand(6, 64)), neg((-w).T.contiguous()).T, neg(-y), neg(-up))):
+        for a, b in zip(want, step(*given)):
+            assert torch.equal(a, b)
+    if dtype == torch.float32:
+        z = torch.complex(torch.zeros_like(h), -h)
+        assert z.conj().imag.is_neg()
+        assert torch.equal(d.linear_cross_entropy(z.conj().imag, w, y), d.linear_cross_entropy(h.clone(), w, y))

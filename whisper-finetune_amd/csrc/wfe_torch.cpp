@@ -135,8 +135,11 @@ Tensor bytes(int64_t n, const Tensor& like) {
 }
 void* pointer(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 
-// t with its last dimension contiguous
-Tensor dense_rows(const Tensor& t) { return t.size(-1) == 1 || t.stride(-1) == 1 ? t : t.contiguous(); }
+// t in memory as it reads: a lazily negated view (torch keeps such for the imaginary part of a conjugate) holds the opposite
+Tensor as_read(const Tensor& t) { return t.is_neg() ? t.resolve_neg() : t; }
+Tensor dense(const Tensor& t) { return as_read(t).contiguous(); }
+// the same with its last dimension contiguous
+Tensor dense_rows(const Tensor& t) { return t.size(-1) == 1 || t.stride(-1) == 1 ? as_read(t) : dense(t); }
 
 // A saved tensor as it was when it was saved, strides apart: hooks on saved tensors may bring back another one.
 void check_saved(const char* name, const Tensor& t, at::IntArrayRef sizes, at::ScalarType type, const c10::Device& device) {
@@ -214,7 +217,7 @@ CeCall ce_forward(Tensor hidden, const Tensor& weight, const Tensor& labels_, in
       stride[levels++] = hidden.stride(i);
     }
   }
-  const Tensor labels = labels_.contiguous();
+  const Tensor labels = dense(labels_);
   wfe_linear_ce& d = c.desc;
   d.device = weight.device().index();
   d.dtype = d.grad_hidden_dtype = d.grad_weight_dtype = dtype_code(weight.scalar_type());
@@ -268,9 +271,9 @@ struct LinearCrossEntropy : torch::autograd::Function<LinearCrossEntropy> {
       const auto types = ctx->saved_data["types"].toIntVector();
       check_saved(kCe, saved[0], {d.vocab, d.dim}, type_of(d.dtype), grads[0].device());
       check_saved(kCe, saved[1], {entry.ce_state(&d)}, at::kByte, grads[0].device());
-      const Tensor weight = dense_rows(saved[0]), state = saved[1].contiguous();
+      const Tensor weight = dense_rows(saved[0]), state = dense(saved[1]);
       d.weight_stride = weight.stride(0);
-      const Tensor upstream = grads[0].to(at::kFloat).contiguous();
+      const Tensor upstream = dense(grads[0].to(at::kFloat));
       Tensor grad_hidden, grad_weight;
       const auto kind = [&](int32_t code) { return code == WFE_F32 ? at::kFloat : weight.scalar_type(); };
       if (ctx->needs_input_grad(0))
@@ -332,7 +335,7 @@ struct EmbedCall {
 EmbedCall embed_forward(const Tensor& ids, const Tensor& weight_, double scale, int64_t padding_idx) {
   EmbedCall c;
   const Tensor weight = dense_rows(weight_);
-  c.ids = ids.contiguous();
+  c.ids = dense(ids);
   wfe_embedding_desc& d = c.desc;
   d.device = weight.device().index();
   d.dtype = d.grad_weight_dtype = dtype_code(weight.scalar_type());
@@ -369,7 +372,7 @@ struct TokenEmbedding : torch::autograd::Function<TokenEmbedding> {
       auto d = unpacked<wfe_embedding_desc>(ctx->saved_data["desc"].toStringRef());
       check_saved(kEmbed, saved, grads[0].sizes().slice(0, grads[0].dim() - 1), d.id_bits == 64 ? at::kLong : at::kInt,
                   grads[0].device());
-      const Tensor ids = saved.contiguous();
+      const Tensor ids = dense(saved);
       Tensor rows = dense_rows(grads[0]);
       if (!rows.is_contiguous()) rows = rows.reshape({-1, d.dim});     // a view where the leading dimensions allow one
       d.grad_stride = rows.is_contiguous() ? d.dim : rows.stride(0);
