@@ -257,7 +257,10 @@ typedef struct {
 
 /* Bytes of the state that the forward pass leaves for the backward pass, and of the workspace of either pass (grads:
  * WFE_GRAD_ bits of the backward pass; weight: the address the pass will get, read by nobody -- rows of W that are
- * no whole multiples of 16 bytes, or not 16-byte aligned, are copied into the workspace).  Both start on 16 bytes.
+ * no whole multiples of 16 bytes, or not 16-byte aligned, are copied into the workspace).  The backward pass takes, beside
+ * that copy, 512 MB at most for the probabilities however many rows there are, 96 MB at most for sums of grad_weight, 64 MB for those
+ * of grad_hidden (many rows: rows by dim in float32, or up to 512 MB), and for WFE_REDUCE_NONE with grad_weight the rows once
+ * more.  State and workspace start on 16 bytes.
  * Negative: a bad description. */
 int64_t wfe_linear_ce_state_bytes(const wfe_linear_ce* d);
 int64_t wfe_linear_ce_workspace_bytes(const wfe_linear_ce* d, const void* weight, int32_t backward, int32_t grads);

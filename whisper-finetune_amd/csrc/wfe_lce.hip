@@ -8,9 +8,9 @@
 // after it runs over the kept rows only, whose number stays on the device.  All four products are one tile routine that
 // multiplies K fragments out of LDS:
 //   STATS  z tiles, reduced in registers to a maximum and a sum of exponentials per row and vocabulary tile
-//   PROB   z tiles again, written as d for a piece of the vocabulary
+//   PROB   z tiles again, written as d for a piece of the vocabulary and, where the rows are many, a share of them
 //   DHID   dh += d W over that piece, in float32
-//   DWEI   the piece's rows of dW, each written once
+//   DWEI   the piece's rows of dW, in float32 until the last share of the rows, then written once
 // Recomputing z costs one product more than keeping (rows, vocab) logits would.
 #include <hip/hip_runtime.h>
 
@@ -255,12 +255,14 @@ struct TileArgs {
   const void* hidden;     // packed rows (row_pad, dim_pad)
   const void* weighted;   // DWEI: the same, or rows times 2^e of their own weight
   const void* weight;     // (vocab, weight_cols) from row v0 on, weight_ld elements apart
-  void* prob;             // d of the piece, (row_pad, prob_ld)
+  void* prob;             // d of the piece, (share, prob_ld)
   long long weight_ld, prob_ld;
   int weight_cols;        // dim, or dim_pad with zeros behind dim; 16-byte rows either way
   int dim, dim_pad, v0, piece, vocab;      // the piece holds vocabulary rows v0 .. v0 + piece - 1
   long long row_pad;
   const int* head;        // [0] kept rows
+  int row0, share;        // kept rows of this call: row0 .. row0 + share - 1, as many of them as there are; what belongs to
+                          // rows (hidden, weighted, label, lse, index, acc) starts at row0
   const int* label;
   float* zlab;
   const float* lse;
@@ -269,11 +271,15 @@ struct TileArgs {
   float2* partial;        // STATS: (vocabulary tiles, row_pad) maximum and sum
   float* acc;             // DHID: (splits, row_pad, dim_pad)
   int first;              // DHID: acc starts with this piece
+  float* wacc;            // DWEI: sums over the shares of the rows so far, (piece, dim_pad)
+  int share_first, share_last;
   void* grad_weight;      // DWEI: (vocab, dim)
   int grad_f32;
   const float* factor;    // DWEI: multiplied with; mean: divided by the number of kept rows
   int mean;
 };
+
+__device__ inline int rows_of(const TileArgs& p) { return max(0, min(p.head[0] - p.row0, p.share)); }
 
 // The id-th of `a_tiles` x `b_tiles` tiles, from column b_first on, of part `split` of `splits` of K.  smem: kLdsBytes.
 template <typename T, class C, int MODE>
@@ -322,8 +328,8 @@ __device__ __forceinline__ void run_tile(const TileArgs& p, int count, int id, i
       la.init(weight, p.weight_ld, a0, p.weight_cols, (long long)k_first * KE, p.piece, wave, lane);
       lb.init(prob, p.prob_ld, b0, b0 + BB, (long long)k_first * KE, 0, wave, lane);
     } else {
-      la.init(static_cast<const T*>(p.weighted), p.dim_pad, a0, p.dim_pad, 0, p.row_pad, wave, lane);
-      lb.init(prob, p.prob_ld, b0, (int)p.prob_ld, 0, p.row_pad, wave, lane);
+      la.init(static_cast<const T*>(p.weighted), p.dim_pad, a0, p.dim_pad, 0, p.share, wave, lane);
+      lb.init(prob, p.prob_ld, b0, (int)p.prob_ld, 0, p.share, wave, lane);
     }
 
 #pragma unroll
@@ -541,7 +547,8 @@ __device__ __forceinline__ void run_tile(const TileArgs& p, int count, int id, i
       }
     }
   } else {
-    const float factor = count > 0 ? *p.factor / (p.mean ? (float)count : 1.f) * (1.f / Elem<T>::kScale) : 0.f;
+    const int all = p.head[0];
+    const float factor = all > 0 ? *p.factor / (p.mean ? (float)all : 1.f) * (1.f / Elem<T>::kScale) : 0.f;
     const bool whole = (p.dim & 3) == 0;
 #pragma unroll
     for (int j = 0; j < FB; ++j) {
@@ -550,11 +557,19 @@ __device__ __forceinline__ void run_tile(const TileArgs& p, int count, int id, i
 #pragma unroll
       for (int i = 0; i < FA; ++i) {
         const int d = a_lane + i * 16;
+        if (d >= p.dim) continue;
+        f32x4 sum = acc[i][j];
+        f32x4* so_far = reinterpret_cast<f32x4*>(p.wacc + (long long)b * p.dim_pad + d);
+        if (!p.share_first) sum += *so_far;
+        if (!p.share_last) {
+          *so_far = sum;
+          continue;
+        }
         const long long at = (long long)(p.v0 + b) * p.dim + d;
-        const f32x4 x = count > 0 ? acc[i][j] * factor : f32x4{0.f, 0.f, 0.f, 0.f};
+        const f32x4 x = all > 0 ? sum * factor : f32x4{0.f, 0.f, 0.f, 0.f};
         if (p.grad_f32) {
           float* out = static_cast<float*>(p.grad_weight) + at;
-          if (whole && d < p.dim) *reinterpret_cast<f32x4*>(out) = x;
+          if (whole) *reinterpret_cast<f32x4*>(out) = x;
           else
             for (int e = 0; e < 4 && d + e < p.dim; ++e) out[e] = x[e];
         } else {
@@ -562,7 +577,7 @@ __device__ __forceinline__ void run_tile(const TileArgs& p, int count, int id, i
           T r[4];
 #pragma unroll
           for (int e = 0; e < 4; ++e) r[e] = static_cast<T>(x[e]);
-          if (whole && d < p.dim) __builtin_memcpy(__builtin_assume_aligned(out, 4 * sizeof(T)), r, sizeof r);
+          if (whole) __builtin_memcpy(__builtin_assume_aligned(out, 4 * sizeof(T)), r, sizeof r);
           else
             for (int e = 0; e < 4 && d + e < p.dim; ++e) out[e] = r[e];
         }
@@ -627,7 +642,7 @@ template <typename T, class C, int MODE>
 __global__ __launch_bounds__(C::kThreads, C::kWavesPerSimd) void lce_logits_kernel(const TileArgs p) {
   extern __shared__ __align__(1024) char smem[];
   int b = blockIdx.x;
-  run_strips<T, C, MODE>(p, p.head[0], b, (p.piece + C::BA - 1) / C::BA, 1, smem);
+  run_strips<T, C, MODE>(p, rows_of(p), b, (p.piece + C::BA - 1) / C::BA, 1, smem);
 }
 
 // DHID has few tiles of its own, so its K, the vocabulary, is split.  Beside DWEI: parts of half a CU's share of all
@@ -657,22 +672,20 @@ __device__ inline int dhid_splits(const SplitRule& r, int count) {
   return best;
 }
 
-// The gradients' products over one piece, and the next piece's d, in one grid: long tiles first, so that the short
+// The gradients' products over one block of d (a piece of the vocabulary, a share of the rows), and the next block's d, in one grid: long tiles first, so that the short
 // ones fill the CUs that run out of them.  (4500 x 1280 x 51866 bfloat16, all but the first of four pieces' d: 1.64 TFLOP in
 // 1.56 ms, 1.06 PFLOP/s.)
 struct GradArgs {
   TileArgs t;
   SplitRule rule;
   int dhid, dwei;
-  int next_v0, next_piece;      // 0: no next piece
-  const void* next_weight;
-  void* next_prob;
+  TileArgs next;                // PROB's; piece 0: no next block
 };
 
 template <typename T, class C>
 __global__ __launch_bounds__(C::kThreads, C::kWavesPerSimd) void lce_grads_kernel(const GradArgs g) {
   extern __shared__ __align__(1024) char smem[];
-  const int count = g.t.head[0];
+  const int count = rows_of(g.t);
   const int dim_tiles = g.rule.dim_tiles;
   int b = blockIdx.x;
   if (g.dwei) {
@@ -685,14 +698,7 @@ __global__ __launch_bounds__(C::kThreads, C::kWavesPerSimd) void lce_grads_kerne
     b -= run_blocks(tiles);
   }
   if (g.dhid && run_strips<T, C, kDhid>(g.t, count, b, dim_tiles, dhid_splits(g.rule, count), smem)) return;
-  if (g.next_piece > 0) {
-    TileArgs p = g.t;
-    p.v0 = g.next_v0;
-    p.piece = g.next_piece;
-    p.weight = g.next_weight;
-    p.prob = g.next_prob;
-    run_strips<T, C, kProb>(p, count, b, (p.piece + C::BA - 1) / C::BA, 1, smem);
-  }
+  if (g.next.piece > 0) run_strips<T, C, kProb>(g.next, rows_of(g.next), b, (g.next.piece + C::BA - 1) / C::BA, 1, smem);
 }
 
 // ---- packing ------------------------------------------------------------------------------------------------
@@ -911,7 +917,7 @@ struct DhidArgs {
   const float* acc;
   SplitRule rule;
   long long row_pad;
-  int rows, dim, dim_pad;
+  int rows, dim, dim_pad, share;
   LceState st;
   const float* upstream;
   int reduction, out_f32;
@@ -926,7 +932,7 @@ __global__ __launch_bounds__(256) void lce_dhid_kernel(const DhidArgs p) {
   const int r = p.st.slot[n], count = p.st.head[0];
   f32x4 s = {0.f, 0.f, 0.f, 0.f};
   if (r >= 0) {
-    const int splits = dhid_splits(p.rule, count);
+    const int splits = dhid_splits(p.rule, min(count - r / p.share * p.share, p.share));
     const bool none = p.reduction == WFE_REDUCE_NONE;
     float g = none ? 1.f / Elem<T>::kScale : *p.upstream * (1.f / Elem<T>::kScale);
     if (p.reduction == WFE_REDUCE_MEAN) g /= (float)count;
@@ -977,15 +983,14 @@ template <typename T> using Tile = std::conditional_t<sizeof(T) == 4, Float, Lar
 template <typename T> using FewTile = std::conditional_t<sizeof(T) == 4, FloatFew, Stream>;
 
 constexpr int kStatsRows = 128;                // fewest vocabulary rows of a tile: room for the statistics
-// What the d of one piece of the vocabulary takes; two are held.  Smaller ones are more launches of fewer tiles each,
-// larger ones leave the cache that a piece's two products read it from (gradients of 4500 x 1280 x 51866 bfloat16: 32 MB
-// 2.30 ms, 128 MB 1.72, 512 MB 2.06).  With many rows a piece of that size is narrow and DWEI's tiles, all rows long, are few:
-// a piece is at least so wide that the three products of a launch keep all CUs busy 1.25 times as long as one tile
-// of DWEI takes, up to kMostPieceBytes (28672 rows of 1280: 128 MB 15.5 ms, 256 to 2048 MB 10.8 to 10.3; of 384: 14.6, at 512
-// 5.1 and 1024 4.7).
-constexpr long long kPieceBytes = 128ll << 20, kMostPieceBytes = 4ll << 30;
-
-template <typename T> using Tile = std::conditional_t<sizeof(T) == 4, Float, Large>;
+// What one block of d takes; two are held.  Smaller ones are more launches of fewer tiles each, larger ones leave the cache
+// that a block's two products read it from (gradients of 4500 x 1280 x 51866 bfloat16: 32 MB 2.30 ms, 128 MB 1.72, 512 MB
+// 2.06).  A block is all rows of a piece of the vocabulary where that makes the piece wide enough: with narrow ones DWEI's
+// tiles, all rows long, are few, and a piece is to be so wide that the three products of a launch keep all CUs busy 1.25
+// times as long as one tile of DWEI takes.  More rows than that are cut into equal shares, over which DWEI's sums are kept in
+// float32, and blocks may be twice as large, fewer shares then reading and writing those sums (loss and gradients of
+// 28672 x 256 x 51866 bfloat16: 4.2 ms, with 128 MB 5.2; 7168 x 64: 0.86 and 0.97).  So d never takes more than 512 MB.
+constexpr long long kBlockBytes = 128ll << 20;
 
 long long up(long long x, long long to) { return (x + to - 1) / to * to; }
 
@@ -994,8 +999,9 @@ struct Plan {
   long long row_pad;
   bool copy_weight;
   int piece, pieces, splits;
+  int share, shares;            // rows of a block
   // offsets into the workspace
-  long long weighted, weight, partial, row_loss, prob[2], acc, top, bytes;
+  long long weighted, weight, partial, row_loss, prob[2], acc, wacc, top, bytes;
 };
 
 template <class C>
@@ -1024,21 +1030,24 @@ Plan make_plan(const wfe_linear_ce& d, const void* weight, bool backward, int gr
     const long long all = up(d.vocab, kLceRowPad);
     const int edge = p.size == 4 ? Float::BB : Large::BB, slots = p.size == 4 ? Float::kSlots : Large::kSlots;
     const long long per_tile = 3 * ((p.dim_pad + edge - 1) / edge);       // tiles of a launch per `edge` of the piece
-    const long long wide = (slots * 5 / 4 + per_tile - 1) / per_tile * edge, row = p.row_pad * p.size;
-    const long long most = kMostPieceBytes / row;
-    long long piece = kPieceBytes / row;
-    if (piece < wide) piece = wide < most ? wide : most;
-    piece = piece / kLceRowPad * kLceRowPad;
-    piece = piece < kLceRowPad ? kLceRowPad : piece;
+    const long long wide = (slots * 5 / 4 + per_tile - 1) / per_tile * edge;
+    const long long columns = (wide < all ? wide : all) * p.size;
+    const long long block = p.row_pad * columns <= kBlockBytes ? kBlockBytes : 2 * kBlockBytes;
+    const long long most = block / columns / kLceRowPad * kLceRowPad;
+    p.shares = (int)((p.row_pad + most - 1) / most);              // (`wide` is 27392 at most, `most` 2304 at least where it cuts)
+    p.share = (int)up((p.row_pad + p.shares - 1) / p.shares, kLceRowPad);      // shares of one size, pieces of one size
+    p.shares = (int)((p.row_pad + p.share - 1) / p.share);
+    const long long piece = block / ((long long)p.share * p.size) / kLceRowPad * kLceRowPad;
     p.pieces = (int)((all + piece - 1) / piece);
-    p.piece = (int)up((all + p.pieces - 1) / p.pieces, kLceRowPad);      // pieces of one size
+    p.piece = (int)up((all + p.pieces - 1) / p.pieces, kLceRowPad);
     p.pieces = (int)((all + p.piece - 1) / p.piece);
     if ((grads & WFE_GRAD_WEIGHT) && d.reduction == WFE_REDUCE_NONE) {
       p.weighted = take(p.row_pad * p.dim_pad * p.size);
       p.top = take(4);
     }
-    p.prob[0] = take(p.row_pad * p.piece * p.size);
-    p.prob[1] = p.pieces > 1 ? take(p.row_pad * p.piece * p.size) : p.prob[0];
+    p.prob[0] = take((long long)p.share * p.piece * p.size);
+    p.prob[1] = p.pieces * p.shares > 1 ? take((long long)p.share * p.piece * p.size) : p.prob[0];
+    if ((grads & WFE_GRAD_WEIGHT) && p.shares > 1) p.wacc = take((long long)p.piece * p.dim_pad * 4);
     if (grads & WFE_GRAD_HIDDEN) {
       const long long one = p.row_pad * p.dim_pad * 4;
       // partial sums of dh: 64 MB; or up to 4 parts in 512 MB, behind which the tiles of one part fill the CUs twice
@@ -1090,6 +1099,7 @@ TileArgs tile_args(const wfe_linear_ce& d, const Plan& p, const void* weight, ch
   a.dim_pad = p.dim_pad;
   a.piece = a.vocab = d.vocab;
   a.row_pad = p.row_pad;
+  a.share = (int)p.row_pad;
   a.head = st.head;
   a.label = st.label;
   a.zlab = st.zlab;
@@ -1170,31 +1180,45 @@ hipError_t gradients(const wfe_linear_ce& d, const Plan& p, GradArgs& g, char* w
   g.rule.slots = C::kSlots;
   g.rule.most = p.splits;
   g.t.prob_ld = p.piece;
-  for (int i = -1; i < p.pieces; ++i) {          // piece i's products beside piece i + 1's d
-    const int v0 = i < 0 ? 0 : i * p.piece, next = (i + 1) * p.piece;
-    g.next_v0 = next;
-    g.next_piece = i + 1 < p.pieces && d.rows > 0 ? (d.vocab - next < p.piece ? d.vocab - next : p.piece) : 0;
-    g.next_weight = w + (long long)next * g.t.weight_ld * p.size;
-    g.next_prob = ws + p.prob[(i + 1) & 1];
-    const long long a_tiles = tiles_of<C>(g.next_piece, true);
-    if (i < 0) {
-      if (d.rows == 0) continue;
-      TileArgs a = g.t;
-      a.v0 = 0;
-      a.piece = g.next_piece;
-      a.prob = g.next_prob;
-      LCE_TRY((launch<T, lce_logits_kernel<T, C, kProb>, C>(a, strip_blocks<C>(a_tiles, d.rows), stream)));
-      continue;
-    }
-    g.t.v0 = v0;
-    g.t.piece = d.vocab - v0 < p.piece ? d.vocab - v0 : p.piece;
-    g.t.weight = w + (long long)v0 * g.t.weight_ld * p.size;
-    g.t.prob = ws + p.prob[i & 1];
-    g.t.first = i == 0;
-    const long long blocks = (g.dwei ? up((long long)g.rule.dim_tiles * tiles_of<C>(g.t.piece, false), 8) : 0) +
-                             (g.dhid ? strip_blocks<C>((long long)g.rule.dim_tiles * p.splits, d.rows) : 0) +
-                             (g.next_piece > 0 ? strip_blocks<C>(a_tiles, d.rows) : 0);
-    if (blocks > 0) LCE_TRY((launch<T, lce_grads_kernel<T, C>, C>(g, blocks, stream)));
+  // Block i: share i % shares of the rows of piece i / shares
+  const auto block = [&](int i) {
+    TileArgs a = g.t;
+    const int v0 = i / p.shares * p.piece, row0 = i % p.shares * p.share;
+    a.v0 = v0;
+    a.piece = d.vocab - v0 < p.piece ? d.vocab - v0 : p.piece;
+    a.weight = w + (long long)v0 * g.t.weight_ld * p.size;
+    a.prob = ws + p.prob[i & 1];
+    a.row0 = row0;
+    a.share = p.share;
+    a.hidden = static_cast<const char*>(g.t.hidden) + (long long)row0 * p.dim_pad * p.size;
+    a.weighted = static_cast<const char*>(g.t.weighted) + (long long)row0 * p.dim_pad * p.size;
+    a.label += row0;
+    a.lse += row0;
+    a.index += row0;
+    a.acc += (long long)row0 * p.dim_pad;
+    a.first = v0 == 0;
+    a.share_first = row0 == 0;
+    a.share_last = i % p.shares == p.shares - 1;
+    return a;
+  };
+  const auto rows_of = [&](const TileArgs& a) { return d.rows - a.row0 < a.share ? d.rows - a.row0 : (int64_t)a.share; };
+  const int blocks = p.pieces * p.shares;
+  if (d.rows > 0) {
+    const TileArgs a = block(0);
+    LCE_TRY((launch<T, lce_logits_kernel<T, C, kProb>, C>(a, strip_blocks<C>(tiles_of<C>(a.piece, true), rows_of(a)), stream)));
+  }
+  const TileArgs base = g.t;
+  for (int i = 0; i < blocks; ++i) {           // block i's products beside block i + 1's d
+    const TileArgs now = block(i);
+    g.next = TileArgs{};
+    if (i + 1 < blocks) g.next = block(i + 1);
+    const long long grid =
+        (g.dwei ? up((long long)g.rule.dim_tiles * tiles_of<C>(now.piece, false), 8) : 0) +
+        (g.dhid ? strip_blocks<C>((long long)g.rule.dim_tiles * p.splits, rows_of(now)) : 0) +
+        (g.next.piece > 0 ? strip_blocks<C>(tiles_of<C>(g.next.piece, true), rows_of(g.next)) : 0);
+    g.t = now;
+    if (grid > 0) LCE_TRY((launch<T, lce_grads_kernel<T, C>, C>(g, grid, stream)));
+    g.t = base;
   }
   return hipSuccess;
 }
@@ -1209,6 +1233,7 @@ hipError_t backward(const wfe_linear_ce& d, const void* weight, const void* stat
   GradArgs g{};
   g.t = tile_args(d, p, weight, ws, st);
   g.t.acc = reinterpret_cast<float*>(ws + p.acc);
+  g.t.wacc = reinterpret_cast<float*>(ws + p.wacc);
   g.t.grad_weight = grad_weight;
   g.t.grad_f32 = d.grad_weight_dtype == WFE_F32;
   g.t.mean = d.reduction == WFE_REDUCE_MEAN;
@@ -1235,6 +1260,7 @@ hipError_t backward(const wfe_linear_ce& d, const void* weight, const void* stat
     k.rows = (int)d.rows;
     k.dim = d.dim;
     k.dim_pad = p.dim_pad;
+    k.share = p.share;
     k.st = st;
     k.upstream = upstream;
     k.reduction = d.reduction;
