@@ -237,7 +237,7 @@ typedef enum { WFE_REDUCE_NONE = 0, WFE_REDUCE_SUM = 1, WFE_REDUCE_MEAN = 2 } wf
 
 /* Softmax cross entropy of labels under logits = hidden @ W^T, the logits never kept:
  *   loss_n = log sum_v exp(h_n . W_v) - h_n . W_{y_n}     (0 where y_n == ignore_index, whatever h_n holds)
- * computed with float32 logits and sums (float32 inputs: products exact to 2^-26 of themselves).  A label outside
+ * computed with float32 logits and sums (float32 inputs: products to 2^-24 of themselves, one rounding).  A label outside
  * 0..vocab-1 that is not ignore_index makes the loss NaN.
  * Hidden row n lies at hidden + (n / inner) * outer_stride + (n % inner) * inner_stride (elements), so that a
  * (batch, length, dim) view is taken as it is; rows of W at weight + v * weight_stride.  dim is contiguous. */
@@ -257,10 +257,10 @@ typedef struct {
 
 /* Bytes of the state that the forward pass leaves for the backward pass, and of the workspace of either pass (grads:
  * WFE_GRAD_ bits of the backward pass; weight: the address the pass will get, read by nobody -- rows of W that are
- * no whole multiples of 16 bytes, or not 16-byte aligned, are copied into the workspace).  The backward pass takes, beside
- * that copy, 512 MB at most for the probabilities however many rows there are, 96 MB at most for sums of grad_weight, 64 MB for those
- * of grad_hidden (many rows: rows by dim in float32, or up to 512 MB), and for WFE_REDUCE_NONE with grad_weight the rows once
- * more.  State and workspace start on 16 bytes.
+ * no whole multiples of 16 bytes, or not 16-byte aligned, are copied into the workspace).  Beside that copy the
+ * backward pass takes 512 MB at most for the probabilities, however many rows there are, 96 MB at most for sums of
+ * grad_weight, 64 MB for those of grad_hidden (many rows: up to 512 MB, or rows by dim in float32), and for
+ * WFE_REDUCE_NONE with grad_weight the rows once more.  State and workspace start on 16 bytes.
  * Negative: a bad description. */
 int64_t wfe_linear_ce_state_bytes(const wfe_linear_ce* d);
 int64_t wfe_linear_ce_workspace_bytes(const wfe_linear_ce* d, const void* weight, int32_t backward, int32_t grads);

@@ -51,8 +51,10 @@ template <> struct Elem<_Float16> {
 };
 // float32 products on the bfloat16 matrix instructions, which do 16 times the work of the float32 ones per cycle: a
 // value is the exact sum of three bfloat16 (8 + 8 + 8 of its 24 bits, each the rounding of what is left), and of the nine
-// partial products the six down to 2^-16 of the whole are added up, smallest first.  What is left out is under 2^-26 of a
-// product, a quarter of what rounding it to float32 costs.  Infinities (inf - inf while splitting) come out as NaN:
+// partial products the six down to 2^-16 of the whole are added up, smallest first.  What is left out, mid lo, lo mid and
+// lo lo with |mid| <= 2^-8 and |lo| <= 2^-17 of a value, is at most 2^-24 (1 + 2^-10) of a product: what rounding it to float32
+// may cost, once.  (Of random values 2^-26 and less in 96 of 100 products.  Two products more would take it to 2^-34, at a
+// third more matrix work.)  Infinities (inf - inf while splitting) come out as NaN:
 // run_tile repeats such a tile with the float32 instructions.
 template <> struct Elem<float> {
   struct Frag { f32x4 x[2]; };
