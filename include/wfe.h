@@ -293,7 +293,8 @@ typedef struct {
 
 int wfe_embedding(const wfe_embedding_desc* d, const void* ids, const void* weight, void* out, void* stream);
 int64_t wfe_embedding_workspace_bytes(const wfe_embedding_desc* d);
-/* grad_weight (vocab, dim) contiguous, fully overwritten. */
+/* grad_weight (vocab, dim) contiguous, fully overwritten.  (rows + 2 vocab) times dim stays under 2^38 in float32 and 2^39 in
+ * half precision, which is more than a device holds, but not more than a grad_stride of 0 can describe. */
 int wfe_embedding_backward(const wfe_embedding_desc* d, const void* ids, const void* grad_out, void* grad_weight,
                            void* workspace, int64_t workspace_bytes, void* stream);
 

@@ -42,7 +42,7 @@ def test_left_out_of_random_products():
 
 def test_left_out_of_the_worst_products():
     one = np.float32(WORST)
-    assert [float(p) for p in split(np.array([one]))] == [1.0, 2.0 ** -8, -2.0 ** -17]
+    assert [float(p[0]) for p in split(np.array([one]))] == [1.0, 2.0 ** -8, -2.0 ** -17]
     assert 0.99 * 2.0 ** -24 < left_out(np.array([one]), np.array([one]))[0] <= LEFT_OUT
     # every value around the ties of the first and the second part, of either sign and some sizes
     near = np.concatenate([np.float32(1 + 2.0 ** -8) + np.arange(-600, 601, dtype=np.float32) * np.float32(2.0 ** -23),

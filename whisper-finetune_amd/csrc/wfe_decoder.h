@@ -52,5 +52,6 @@ hipError_t launch_embedding(const wfe_embedding_desc& d, const void* ids, const 
 hipError_t launch_embedding_backward(const wfe_embedding_desc& d, const void* ids, const void* grad_out,
                                      void* grad_weight, void* workspace, hipStream_t stream);
 int64_t embedding_workspace_bytes(const wfe_embedding_desc& d);
+bool embedding_backward_fits(const wfe_embedding_desc& d);      // a launch has fewer than 2^32 threads
 
 }  // namespace wfe

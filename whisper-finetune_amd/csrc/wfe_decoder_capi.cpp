@@ -174,6 +174,9 @@ int64_t wfe_embedding_workspace_bytes(const wfe_embedding_desc* d) {
 int wfe_embedding_backward(const wfe_embedding_desc* d, const void* ids, const void* grad_out, void* grad_weight,
                            void* workspace, int64_t workspace_bytes, void* stream) {
   CHECKED(check_embedding(d));
+  if (!wfe::embedding_backward_fits(*d))
+    return wfe::fail(nullptr, WFE_ERR_ARG, "embedding: the gradient of %lld rows, %d of the vocabulary and dim %d is more than one "
+                     "launch", (long long)d->rows, d->vocab, d->dim);
   if (!grad_weight || (d->rows > 0 && (!ids || !grad_out)))
     return wfe::fail(nullptr, WFE_ERR_ARG, "embedding: null device pointer");
   if (!aligned(ids, d->id_bits / 8) || !aligned(grad_out, size_of(d->dtype)) || !aligned(grad_weight, 16))

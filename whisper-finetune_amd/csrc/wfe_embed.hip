@@ -373,14 +373,21 @@ hipError_t embed(const wfe_embedding_desc& d, const void* ids, const void* weigh
              : embed_as<T, false>(d, ids, weight, out, stream);
 }
 
+// Blocks of the sums' launch: a wave per piece and slab, then a wave per kRowsPerWave rows of the vocabulary and slab
+struct SumGrid {
+  int64_t pieces, rows;
+};
+SumGrid sum_grid(int64_t pieces, int64_t vocab, int64_t slabs) {
+  return {(pieces * slabs + 3) / 4, ((vocab + kRowsPerWave - 1) / kRowsPerWave * slabs + 3) / 4};
+}
+
 template <typename T, bool WIDE>
 hipError_t sums_as(const SumArgs& p, hipStream_t stream) {
   constexpr int kSlab = 64 * (16 / (int)sizeof(T));
   const unsigned slabs = (p.dim + kSlab - 1) / kSlab;
-  const int64_t piece_blocks = ((int64_t)p.pieces * slabs + 3) / 4;
-  const int64_t row_blocks = (((int64_t)p.vocab + kRowsPerWave - 1) / kRowsPerWave * slabs + 3) / 4;
-  embed_sum_kernel<T, WIDE><<<dim3((unsigned)(piece_blocks + row_blocks)), dim3(256), 0, stream>>>(
-      p, (int)piece_blocks, (int)slabs);
+  const SumGrid grid = sum_grid(p.pieces, p.vocab, slabs);
+  embed_sum_kernel<T, WIDE><<<dim3((unsigned)(grid.pieces + grid.rows)), dim3(256), 0, stream>>>(
+      p, (int)grid.pieces, (int)slabs);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess || p.pieces == 0) return e;
   embed_join_kernel<T, WIDE><<<dim3((p.pieces + kJoinPieces - 1) / kJoinPieces, slabs), dim3(kJoinWaves * 64), 0,
@@ -419,6 +426,12 @@ hipError_t embed_backward(const wfe_embedding_desc& d, const void* ids, const vo
 
 int64_t embedding_workspace_bytes(const wfe_embedding_desc& d) {
   return index_bytes(d) + pieces_of(d) * 2 * (int64_t)d.dim * 4;
+}
+
+bool embedding_backward_fits(const wfe_embedding_desc& d) {
+  const int64_t slab = 64 * (d.dtype == WFE_F32 ? 4 : 8);
+  const SumGrid grid = sum_grid(pieces_of(d), d.vocab, (d.dim + slab - 1) / slab);
+  return (grid.pieces + grid.rows) * 256 < (int64_t)1 << 32;
 }
 
 hipError_t launch_embedding(const wfe_embedding_desc& d, const void* ids, const void* weight, void* out,
