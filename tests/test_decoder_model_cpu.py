@@ -254,3 +254,41 @@ def test_installed_models_pickle_and_save_whole(plain, tmp_path):
     assert torch.allclose(again(**batch()).loss, want.loss, atol=1e-6)
     with pytest.raises(AttributeError):
         decoder.no_such_name
+
+
+def trainer_losses(model, tmp_path, **kw):
+    """Two steps of the Seq2SeqTrainer that finetune.py uses, on batches as the collator makes them; -> losses, weights."""
+    from transformers import Seq2SeqTrainer, Seq2SeqTrainingArguments
+    torch.manual_seed(0)
+    data = [{k: v[i] for k, v in batch(s).items()} for s in range(4) for i in range(2)]
+    args = Seq2SeqTrainingArguments(output_dir=str(tmp_path), per_device_train_batch_size=2, max_steps=2, logging_steps=1,
+                                    learning_rate=1e-3, report_to=[], save_strategy="no", disable_tqdm=True,
+                                    dataloader_pin_memory=False, remove_unused_columns=False, **kw)
+    trainer = Seq2SeqTrainer(model=model, args=args, train_dataset=data, eval_dataset=data,
+                             data_collator=lambda rows: {k: torch.stack([r[k] for r in rows]) for k in rows[0]})
+    trainer.train()
+    losses = [e["loss"] for e in trainer.state.log_history if "loss" in e]
+    return trainer, losses
+
+
+def test_trainer_steps_and_evaluation(plain, tmp_path):
+    stock, model = pair()
+    decoder.install(model, logits_in_eval=False)
+    (_, want), (trainer, got) = (trainer_losses(m, tmp_path, use_cpu=True) for m in (stock, model))
+    assert len(want) == 2 and got == pytest.approx(want, abs=1e-4)
+    for (name, p), q in zip(stock.named_parameters(), model.named_parameters()):
+        assert torch.allclose(p, q[1], atol=1e-4), name
+    # a Trainer's predictions: nothing passes for logits (of 103 columns) that is none
+    found = trainer.predict(trainer.eval_dataset)
+    flat = found.predictions if isinstance(found.predictions, tuple) else (found.predictions,)
+    assert all(getattr(x, "shape", (0,))[-1] != 16 or x.shape[1] == 10 for x in flat if x is not None)     # (the encoder's states)
+
+
+def test_losses_may_be_added_to_in_place(plain):
+    """As adapter libraries do with their regularisation."""
+    _, model = pair()
+    out = model(**batch())
+    out.loss += 2.0
+    assert out["loss"] is out.loss and out[0] is out.loss
+    out.loss.backward()
+    assert model.get_output_embeddings().weight.grad is not None
