@@ -148,25 +148,26 @@ void check_saved(const char* name, const Tensor& t, at::IntArrayRef sizes, at::S
                              "or device (from hooks on saved tensors)");
 }
 
-// Refuses to record a call on parameters that a graph of an earlier call, still alive, holds on to.  Autograd keeps one
-// accumulation node per parameter while any graph refers to it, on the stream it was made on; a captured backward pass
-// would draw that stream into the capture, never to leave it, which ends the process.
+// Refuses to record a call on parameters that a graph of an earlier call on the default stream, still alive, holds on to.
+// Autograd keeps one accumulation node per parameter while any graph refers to it, on the stream it was made on; a captured
+// backward pass would make that stream wait for the capture.  Another stream is drawn into the capture and joined again at
+// the pass's end (warming up on a side stream is how a capture is prepared); the default stream cannot be, which ends the
+// process.
 void check_capture(const char* name, std::initializer_list<Tensor> inputs) {
   for (const Tensor& t : inputs) {
     if (!t.requires_grad() || !t.is_leaf()) continue;
     const auto node = torch::autograd::impl::try_get_grad_accumulator(t);
     if (!node) continue;
     const auto made_on = node->stream();
-    const auto stream = stream_of(t);
-    if (!made_on || made_on->id() == stream.id()) continue;
+    if (!made_on || made_on->id() != c10::hip::getDefaultHIPStream(t.device().index()).id()) continue;
     hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
-    if (hipStreamIsCapturing(static_cast<hipStream_t>(raw(stream)), &status) != hipSuccess) {
+    if (hipStreamIsCapturing(static_cast<hipStream_t>(raw(stream_of(t))), &status) != hipSuccess) {
       (void)hipGetLastError();
       continue;
     }
     if (status == hipStreamCaptureStatusNone) continue;
-    throw std::runtime_error(std::string(name) + ": captured while the autograd graph of an earlier call with the same "
-                             "parameter is alive; drop that call's results (or detach them) before capturing");
+    throw std::runtime_error(std::string(name) + ": captured while the autograd graph of an earlier call on the default stream "
+                             "with the same parameter is alive; drop that call's results (or detach them) before capturing");
   }
 }
 

@@ -7,8 +7,8 @@
   (the Seq2SeqTrainer of finetune.py:144-150 calls ``model(**batch)`` with the collator's labels) then runs on them.
 
 They work on the current stream of the tensors' device, allocate their workspace from torch's allocator and never
-synchronise, so they can be captured into a graph (not while the graph of an earlier call over the same parameters is
-alive: that is refused, since torch would end the process).  There is no CPU path: tensors elsewhere raise.
+synchronise, so they can be captured into a graph (not while the graph of an earlier call on the default
+stream over the same parameters is alive: that is refused, since torch would end the process).  There is no CPU path: tensors elsewhere raise.
 
 The kernels and their C ABI are in libwfe_hip.so; ``_decoder.so`` (csrc/wfe_torch.cpp) makes them differentiable.
 """
