@@ -269,7 +269,8 @@ int wfe_linear_ce_forward(const wfe_linear_ce* d, const void* hidden, const void
                           float* loss, void* state, void* workspace, int64_t workspace_bytes, void* stream);
 /* upstream: float32 gradient of `loss` (as many entries as it).  grad_hidden (rows, dim) and grad_weight
  * (vocab, dim), contiguous, fully overwritten; either may be NULL.  weight and state as in the forward pass (the
- * state holds the rows of hidden that count). */
+ * state holds the rows of hidden that count; weight may lie elsewhere, with its weight_stride).  float16 with
+ * WFE_REDUCE_NONE: a row enters grad_weight to 2^-24 of the largest |upstream|. */
 int wfe_linear_ce_backward(const wfe_linear_ce* d, const void* weight, const void* state, const float* upstream,
                            void* grad_hidden, void* grad_weight, void* workspace, int64_t workspace_bytes,
                            void* stream);

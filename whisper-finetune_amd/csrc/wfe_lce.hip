@@ -103,6 +103,8 @@ template <typename T> constexpr int kKBytes = kKElems * (int)sizeof(T);
 constexpr int kPadRows = 64;                               // zeros follow the kept rows up to a multiple of this
 constexpr float kLog2e = 1.44269504088896340736f;
 
+// (The argument's rounding, half a step of x log2(e), is what a logit's own rounding may be; the loss of 16-bit inputs is off
+// by 0.7e-6 at a dim of 384 and 1.2e-6 at 1280, root mean square.)
 __device__ inline float exp_of(float x) { return __builtin_amdgcn_exp2f(x * kLog2e); }
 
 // A row's own weight as m 2^e, 1 <= |m| < 2 (or 0, an infinity, NaN): m goes into d before that is rounded, 2^e where it costs no
@@ -674,9 +676,9 @@ __device__ inline int dhid_splits(const SplitRule& r, int count) {
   return best;
 }
 
-// The gradients' products over one block of d (a piece of the vocabulary, a share of the rows), and the next block's d, in one grid: long tiles first, so that the short
-// ones fill the CUs that run out of them.  (4500 x 1280 x 51866 bfloat16, all but the first of four pieces' d: 1.64 TFLOP in
-// 1.56 ms, 1.06 PFLOP/s.)
+// The gradients' products over one block of d (a piece of the vocabulary, a share of the rows), and the next block's d, in
+// one grid: long tiles first, so that the short ones fill the CUs that run out of them.  (4500 x 1280 x 51866 bfloat16, all
+// but the first of four blocks' d: 1.64 TFLOP in 1.56 ms, 1.06 PFLOP/s.)
 struct GradArgs {
   TileArgs t;
   SplitRule rule;

@@ -7,8 +7,9 @@
   (the Seq2SeqTrainer of finetune.py:144-150 calls ``model(**batch)`` with the collator's labels) then runs on them.
 
 They work on the current stream of the tensors' device, allocate their workspace from torch's allocator and never
-synchronise, so they can be captured into a graph (not while the graph of an earlier call on the default
-stream over the same parameters is alive: that is refused, since torch would end the process).  There is no CPU path: tensors elsewhere raise.
+synchronise, so they can be captured into a graph (not while the graph of an earlier call on the default stream over the
+same parameters is alive: that is refused, since torch would end the process).  There is no CPU path: tensors elsewhere
+raise.
 
 The kernels and their C ABI are in libwfe_hip.so; ``_decoder.so`` (csrc/wfe_torch.cpp) makes them differentiable.
 """
@@ -148,10 +149,10 @@ def __getattr__(name):
 def install(model, logits_in_eval: bool = True):
     """Puts the two operators into ``model``, a ``WhisperForConditionalGeneration`` (or a wrapper whose
     ``get_base_model()`` is one), in place, and returns it: the decoder's token embedding, and the loss of a call with
-    ``labels``.  Such a call returns its loss and no logits (``logits`` is None); in evaluation mode it computes both
-    as before unless ``logits_in_eval`` is False.  Calls without labels, generation, copies and saved files are as
-    before, and so is everything while the weights are on the CPU or in 64 bits.  Installing twice only sets
-    ``logits_in_eval``."""
+    ``labels``.  Such a call returns its loss and no logits (no such entry); in evaluation mode it computes both
+    as before unless ``logits_in_eval`` is False.  Calls without labels or for tuples, generation, copies, pickles and
+    saved files are as before, and so is everything while the weights are on the CPU or in 64 bits, or the output
+    projection is another module than it was, or hooked.  Installing twice only sets ``logits_in_eval``."""
     base = model.get_base_model() if hasattr(model, "get_base_model") else model
     from transformers import WhisperForConditionalGeneration
     if isinstance(base, _model_class()):
